@@ -67,7 +67,8 @@ const char* marlin_q4_status_string(int status);
 /* cudaError_t of the last failed launch in this thread (0 if none). */
 int marlin_q4_last_cuda_error(void);
 /* Device-side error word of the current device (0 = none; 1 = a bounded wait timed out, on this
- * GPU's own copies or on a peer's exchange words; 3 = an embedding id out of range).
+ * GPU's own copies or on a peer's exchange words; 3 = an index out of range: an embedding id, a
+ * cache slot, a page of a block table, a sequence's start or length).
  * Synchronous: copies the word to the host.  clear != 0 resets it to 0.  While the word is set,
  * the exchange waits of marlin_q4_tp_decode_step return at once (see there): clear it before the
  * next step once the ranks are known to be in step again. */
@@ -264,6 +265,83 @@ int marlin_q4_ipc_close_handle(void* ptr);
  * rounded once (round to nearest even).  ids: int32 [m] on the device; out: bf16 [m, table->k],
  * 16-byte aligned.  An id outside [0, table->n) yields a zero row and device error 3. */
 int marlin_q4_embed(const int32_t* ids, int64_t m, const marlin_q4_tensor* table, uint16_t* out, void* stream);
+
+/* ---- attention around a quantized, paged key/value cache ------------------------------------------
+ * The operators between the projections of a gated-attention layer (src/model/attention.cpp:82-139:
+ * head norms, rotary positions, cache append, attention) for serving: forward only.  head_dim 64,
+ * 128 or 256; at most 2^24 tokens per call; tokens == 0 returns MARLIN_Q4_OK without a launch.
+ *
+ * Cache: [pages][kv_heads][page_size / 16] units of marlin_q4_kv_unit_bytes bytes, each 16 consecutive
+ * positions of one head: key codes, key {scale, bias} pairs, value codes, value pairs.  The format is
+ * the weights' (groups of 64 features, value = scale * code + bias, scale and bias bf16), bits 4 or 8.
+ * page_size: a multiple of 16, at most 4096; pages * page_size < 2^31; data 16-byte aligned.
+ * Position p of a sequence lies in page block_table[sequence][p / page_size], row p % page_size; the
+ * slot of that row is page * page_size + p % page_size. */
+typedef struct marlin_q4_kv_cache {
+    void* data;
+    int64_t pages;
+    int32_t page_size;
+    int32_t kv_heads;
+    int32_t head_dim;
+    int32_t bits;
+} marlin_q4_kv_cache;
+/* Bytes of one unit (16 positions of one head); 0 for a head_dim or bits outside the above. */
+size_t marlin_q4_kv_unit_bytes(int32_t head_dim, int32_t bits);
+
+/* Head norms and rotary positions in one pass: for each token and each row x of q's heads (k's
+ * kv_heads), n = x * rsqrt(mean(x^2) + eps) * (1 + w), then the rot_dim / 2 pairs of its first rot_dim
+ * features turn by angle = position * inv_freq: (a, b) -> (a cos - b sin, b cos + a sin).  Pairs are
+ * (i, i + rot_dim / 2), or (2i, 2i + 1) when interleaved != 0.  All in binary32 (the angle in binary64),
+ * rounded once to out_dtype.
+ * q, k: [tokens, heads | kv_heads, head_dim] of x_dtype, features contiguous, token and head strides in
+ * elements (multiples of 16 bytes; both pointers 16-byte aligned), so the projections need no copy.
+ * positions: int32 [axes, tokens], axes 1 to 4; axis_of: HOST array of rot_dim / 2 axis numbers, one per
+ * pair (multi-axis positions of image patches), or NULL for axis 0.  inv_freq: binary32 [rot_dim / 2] on
+ * the device, with whatever scaling for long contexts the caller chose.  rot_dim: a multiple of 16, at
+ * most head_dim.  q_weight, k_weight: bf16 [head_dim], 16-byte aligned.  q_out, k_out: contiguous
+ * [tokens, heads | kv_heads, head_dim], 16-byte aligned, not overlapping the inputs. */
+int marlin_q4_qk_norm_rope(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
+                           int64_t k_token_stride, int64_t k_head_stride, int32_t x_dtype, int64_t tokens,
+                           int32_t heads, int32_t kv_heads, int32_t head_dim, const uint16_t* q_weight,
+                           const uint16_t* k_weight, float eps, const int32_t* positions, int32_t axes,
+                           const uint8_t* axis_of, const float* inv_freq, int32_t rot_dim, int32_t interleaved,
+                           void* q_out, void* k_out, int32_t out_dtype, void* stream);
+
+/* Write keys and values of `tokens` tokens into the cache, quantized on the way by the rule of
+ * marlin_q4_quantize (15 or 255 steps) on their values rounded to bf16.  k, v: [tokens, kv_heads,
+ * head_dim] of x_dtype, finite, strides as above.  slots: int32 [tokens]; a negative slot skips its
+ * token (padding), one outside the pool skips it and sets device error 3.  The slots >= 0 of one call
+ * must differ: two tokens on one slot leave its row a mix of both. */
+int marlin_q4_kv_write(const marlin_q4_kv_cache* cache, const void* k, int64_t k_token_stride,
+                       int64_t k_head_stride, const void* v, int64_t v_token_stride, int64_t v_head_stride,
+                       int32_t x_dtype, const int32_t* slots, int64_t tokens, void* stream);
+/* Read rows back: k, v: bf16 [tokens, kv_heads, head_dim], 16-byte aligned, bf16(scale * code + bias)
+ * with one rounding.  A negative slot gives a zero row; one outside the pool too, and device error 3. */
+int marlin_q4_kv_read(const marlin_q4_kv_cache* cache, const int32_t* slots, int64_t tokens, uint16_t* k,
+                      uint16_t* v, void* stream);
+
+/* Causal attention of each sequence's newest tokens over the cache (their own keys and values already
+ * written): out = softmax(scale * q K^T) V per head, query head i reading kv head i / (heads / kv_heads).
+ * Sequence b has kv_lens[b] cached positions and owns the q rows [cu_q[b], cu_q[b + 1]) (int32
+ * [batch + 1], ascending), at most max_q of them; its last row sees all positions, the one before it one
+ * less, and so on.  A row that sees none is zero; rows of q outside every sequence are left as they were
+ * in out.  cu_q NULL: one row per sequence (tokens == batch, max_q ignored).
+ * q: bf16 [tokens, heads, head_dim], strides as above; out: bf16, contiguous, 16-byte aligned.
+ * block_table: int32 [batch, table_width], rows table_stride elements apart; entries behind a
+ * sequence's last page are not read.  heads: a multiple of kv_heads; batch at most 1024; scale > 0.
+ * K and V are rounded to bf16, softmax weights too (for the tensor cores); sums are binary32.
+ * A page outside the pool, a start or length outside its range sets device error 3, and the rows of that
+ * sequence are void (no access leaves the buffers).
+ * workspace: >= marlin_q4_paged_attention_workspace_size bytes, 256-byte aligned, any content; calls
+ * that may overlap in time need one each. */
+int marlin_q4_paged_attention(const uint16_t* q, int64_t q_token_stride, int64_t q_head_stride,
+                              const marlin_q4_kv_cache* cache, int64_t tokens, int32_t heads,
+                              const int32_t* block_table, int64_t table_stride, int32_t table_width,
+                              const int32_t* kv_lens, const int32_t* cu_q, int32_t batch, int32_t max_q,
+                              float scale, uint16_t* out, void* workspace, size_t workspace_bytes, void* stream);
+/* 0 for arguments outside the above. */
+size_t marlin_q4_paged_attention_workspace_size(int64_t tokens, int32_t heads, int32_t kv_heads,
+                                                int32_t head_dim, int32_t batch);
 
 /* ---- synthetic inputs (benchmark / test support; no counterpart in the reference) ----------------
  * out[i] = bf16(mean + sigma * z_i), z_i a seeded Irwin-Hall(12) variate (mean 0, sd 1), the same

@@ -5,6 +5,7 @@
 // marlin_q4_device_error, which is documented as synchronous) and never allocates.
 #include "marlin_q4.h"
 
+#include "kv_cache.cuh"
 #include "q4_fused.cuh"
 #include "q4_gemv.cuh"
 #include "q4_i8.cuh"
@@ -61,6 +62,33 @@ int check_act16(const void* x, int32_t dtype) {
 }
 
 int check_norm(const uint16_t* w) { return (!w || aligned(w, 16)) ? MARLIN_Q4_OK : MARLIN_Q4_ERR_ALIGN; }
+
+bool kv_dims(int32_t head_dim, int32_t bits) {
+    return (head_dim == 64 || head_dim == 128 || head_dim == 256) && (bits == 4 || bits == 8);
+}
+
+constexpr int64_t kMaxTokens = (int64_t)1 << 24;
+constexpr int32_t kMaxHeads = 1024;
+
+int check_cache(const marlin_q4_kv_cache* c) {
+    if (!c || !c->data || c->pages <= 0 || c->kv_heads <= 0) return MARLIN_Q4_ERR_ARG;
+    if (c->page_size <= 0 || c->page_size % 16 != 0) return MARLIN_Q4_ERR_SHAPE;
+    if (!kv_dims(c->head_dim, c->bits) || c->page_size > 4096 || c->kv_heads > kMaxHeads ||
+        c->pages > INT32_MAX / c->page_size)
+        return MARLIN_Q4_ERR_UNSUPPORTED;
+    return aligned(c->data, 16) ? MARLIN_Q4_OK : MARLIN_Q4_ERR_ALIGN;
+}
+
+KvPool view(const marlin_q4_kv_cache* c) {
+    return KvPool{static_cast<uint8_t*>(c->data), c->pages, c->page_size / 16, c->kv_heads, c->head_dim, c->bits};
+}
+
+// a strided [tokens, heads, head_dim] operand read with 16-byte loads
+int check_heads(const void* x, int32_t dtype, int64_t token_stride, int64_t head_stride) {
+    if (!x || !valid_dtype(dtype) || token_stride < 0 || head_stride < 0) return MARLIN_Q4_ERR_ARG;
+    const int64_t per = 16 / (int64_t)dtype_size(dtype);
+    return aligned(x, 16) && token_stride % per == 0 && head_stride % per == 0 ? MARLIN_Q4_OK : MARLIN_Q4_ERR_ALIGN;
+}
 
 Q4Mat view(const marlin_q4_tensor* t) { return Q4Mat{t->weight, t->scales, t->biases, t->n, t->k}; }
 
@@ -140,12 +168,15 @@ int marlin_q4_device_error(int clear) {
     int v = gemv_device_error(clear != 0);
     const int v_i8 = i8_device_error(clear != 0), v_pf = prefill_device_error(clear != 0),
               v_mi = misc_device_error(clear != 0), v_fu = fused_device_error(clear != 0),
-              v_ro = rows_device_error(clear != 0);
+              v_ro = rows_device_error(clear != 0), v_kv = kv_device_error(clear != 0),
+              v_at = attn_device_error(clear != 0);
     if (!v) v = v_fu;
     if (!v) v = v_ro;
     if (!v) v = v_i8;
     if (!v) v = v_pf;
     if (!v) v = v_mi;
+    if (!v) v = v_kv;
+    if (!v) v = v_at;
     if (v < 0) return cuda_status(cudaGetLastError());
     return v;
 }
@@ -210,6 +241,139 @@ int marlin_q4_embed(const int32_t* ids, int64_t m, const marlin_q4_tensor* table
     if (!aligned(ids, 4) || !aligned(out, 16)) return MARLIN_Q4_ERR_ALIGN;
     return cuda_status(launch_embed_q4(ids, m, table->weight, table->scales, table->biases, table->n, table->k, out,
                                        static_cast<cudaStream_t>(stream)));
+}
+
+size_t marlin_q4_kv_unit_bytes(int32_t head_dim, int32_t bits) {
+    return kv_dims(head_dim, bits) ? (size_t)kv_unit_bytes(head_dim, bits) : 0;
+}
+
+int marlin_q4_qk_norm_rope(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k,
+                           int64_t k_token_stride, int64_t k_head_stride, int32_t x_dtype, int64_t tokens,
+                           int32_t heads, int32_t kv_heads, int32_t head_dim, const uint16_t* q_weight,
+                           const uint16_t* k_weight, float eps, const int32_t* positions, int32_t axes,
+                           const uint8_t* axis_of, const float* inv_freq, int32_t rot_dim, int32_t interleaved,
+                           void* q_out, void* k_out, int32_t out_dtype, void* stream) {
+    if (tokens < 0 || heads <= 0 || kv_heads <= 0 || axes < 1 || axes > 4 || !valid_dtype(out_dtype))
+        return MARLIN_Q4_ERR_ARG;
+    if (head_dim != 64 && head_dim != 128 && head_dim != 256) return MARLIN_Q4_ERR_UNSUPPORTED;
+    if (rot_dim <= 0 || rot_dim % 16 != 0 || rot_dim > head_dim) return MARLIN_Q4_ERR_SHAPE;
+    if (tokens > kMaxTokens || heads > kMaxHeads || kv_heads > kMaxHeads) return MARLIN_Q4_ERR_UNSUPPORTED;
+    RopeArgs a{};
+    for (int i = 0; axis_of && i < rot_dim / 2; ++i) {
+        if (axis_of[i] >= axes) return MARLIN_Q4_ERR_ARG;
+        a.axis[i / 16] |= (uint32_t)axis_of[i] << (i % 16 * 2);
+    }
+    if (tokens == 0) return MARLIN_Q4_OK;
+    int rc;
+    if ((rc = check_heads(q, x_dtype, q_token_stride, q_head_stride)) ||
+        (rc = check_heads(k, x_dtype, k_token_stride, k_head_stride)))
+        return rc;
+    if (!q_weight || !k_weight || !positions || !inv_freq || !q_out || !k_out) return MARLIN_Q4_ERR_ARG;
+    if (!aligned(q_weight, 16) || !aligned(k_weight, 16) || !aligned(q_out, 16) || !aligned(k_out, 16) ||
+        !aligned(positions, 4) || !aligned(inv_freq, 4))
+        return MARLIN_Q4_ERR_ALIGN;
+    a.q = q;
+    a.k = k;
+    a.q_ts = q_token_stride;
+    a.q_hs = q_head_stride;
+    a.k_ts = k_token_stride;
+    a.k_hs = k_head_stride;
+    a.tokens = tokens;
+    a.heads = heads;
+    a.kv_heads = kv_heads;
+    a.dim = head_dim;
+    a.qw = q_weight;
+    a.kw = k_weight;
+    a.eps = eps;
+    a.positions = positions;
+    a.freqs = inv_freq;
+    a.rot = rot_dim;
+    a.interleaved = interleaved != 0;
+    a.q_out = q_out;
+    a.k_out = k_out;
+    return cuda_status(launch_qk_norm_rope(a, x_dtype, out_dtype, g_pdl, static_cast<cudaStream_t>(stream)));
+}
+
+int marlin_q4_kv_write(const marlin_q4_kv_cache* cache, const void* k, int64_t k_token_stride, int64_t k_head_stride,
+                       const void* v, int64_t v_token_stride, int64_t v_head_stride, int32_t x_dtype,
+                       const int32_t* slots, int64_t tokens, void* stream) {
+    int rc = check_cache(cache);
+    if (rc) return rc;
+    if (tokens < 0) return MARLIN_Q4_ERR_ARG;
+    if (tokens > kMaxTokens) return MARLIN_Q4_ERR_UNSUPPORTED;
+    if (tokens == 0) return MARLIN_Q4_OK;
+    if ((rc = check_heads(k, x_dtype, k_token_stride, k_head_stride)) ||
+        (rc = check_heads(v, x_dtype, v_token_stride, v_head_stride)))
+        return rc;
+    if (!slots) return MARLIN_Q4_ERR_ARG;
+    if (!aligned(slots, 4)) return MARLIN_Q4_ERR_ALIGN;
+    return cuda_status(launch_kv_write(view(cache), k, k_token_stride, k_head_stride, v, v_token_stride, v_head_stride,
+                                       x_dtype, slots, tokens, g_pdl, static_cast<cudaStream_t>(stream)));
+}
+
+int marlin_q4_kv_read(const marlin_q4_kv_cache* cache, const int32_t* slots, int64_t tokens, uint16_t* k, uint16_t* v,
+                      void* stream) {
+    const int rc = check_cache(cache);
+    if (rc) return rc;
+    if (tokens < 0) return MARLIN_Q4_ERR_ARG;
+    if (tokens > kMaxTokens) return MARLIN_Q4_ERR_UNSUPPORTED;
+    if (tokens == 0) return MARLIN_Q4_OK;
+    if (!slots || !k || !v) return MARLIN_Q4_ERR_ARG;
+    if (!aligned(slots, 4) || !aligned(k, 16) || !aligned(v, 16)) return MARLIN_Q4_ERR_ALIGN;
+    return cuda_status(launch_kv_read(view(cache), slots, tokens, k, v, g_pdl, static_cast<cudaStream_t>(stream)));
+}
+
+size_t marlin_q4_paged_attention_workspace_size(int64_t tokens, int32_t heads, int32_t kv_heads, int32_t head_dim,
+                                                int32_t batch) {
+    if (tokens < 0 || tokens > kMaxTokens || heads <= 0 || heads > kMaxHeads || kv_heads <= 0 || heads % kv_heads != 0 ||
+        !kv_dims(head_dim, 4) || batch <= 0 || batch > kAttnMaxBatch)
+        return 0;
+    return align16(attn_workspace_bytes(tokens, heads, kv_heads, head_dim, batch));
+}
+
+int marlin_q4_paged_attention(const uint16_t* q, int64_t q_token_stride, int64_t q_head_stride,
+                              const marlin_q4_kv_cache* cache, int64_t tokens, int32_t heads,
+                              const int32_t* block_table, int64_t table_stride, int32_t table_width,
+                              const int32_t* kv_lens, const int32_t* cu_q, int32_t batch, int32_t max_q, float scale,
+                              uint16_t* out, void* workspace, size_t workspace_bytes, void* stream) {
+    int rc = check_cache(cache);
+    if (rc) return rc;
+    if (tokens < 0 || heads <= 0 || batch < 0 || table_width < 0 || table_stride < 0) return MARLIN_Q4_ERR_ARG;
+    if (!(scale > 0.f) || !(scale <= 3.0e38f)) return MARLIN_Q4_ERR_ARG;
+    if (heads % cache->kv_heads != 0) return MARLIN_Q4_ERR_SHAPE;
+    if (!cu_q && tokens != batch) return MARLIN_Q4_ERR_SHAPE;
+    if (cu_q && max_q < 0) return MARLIN_Q4_ERR_ARG;
+    if (tokens > kMaxTokens || heads > kMaxHeads || batch > kAttnMaxBatch ||
+        table_width > INT32_MAX / cache->page_size)
+        return MARLIN_Q4_ERR_UNSUPPORTED;
+    if (tokens == 0 || batch == 0 || (cu_q && max_q == 0)) return MARLIN_Q4_OK;
+    if ((rc = check_heads(q, MARLIN_Q4_BF16, q_token_stride, q_head_stride))) return rc;
+    if (!kv_lens || !out || (!block_table && table_width > 0)) return MARLIN_Q4_ERR_ARG;
+    if (!aligned(block_table, 4) || !aligned(kv_lens, 4) || !aligned(cu_q, 4) || !aligned(out, 16)) return MARLIN_Q4_ERR_ALIGN;
+    if (!workspace || !aligned(workspace, 256) ||
+        workspace_bytes < marlin_q4_paged_attention_workspace_size(tokens, heads, cache->kv_heads, cache->head_dim, batch))
+        return MARLIN_Q4_ERR_WORKSPACE;
+    AttnArgs a{};
+    a.q = q;
+    a.q_ts = q_token_stride;
+    a.q_hs = q_head_stride;
+    a.pool = view(cache);
+    a.tokens = tokens;
+    a.heads = heads;
+    a.group = heads / cache->kv_heads;
+    a.table = block_table;
+    a.table_stride = table_stride;
+    a.table_width = table_width;
+    a.kv_lens = kv_lens;
+    a.cu_q = cu_q;
+    a.batch = batch;
+    a.max_q = cu_q ? (int)std::min<int64_t>(max_q, tokens) : 1;
+    a.scale_log2 = scale * 1.4426950408889634f;
+    a.out = out;
+    a.part = static_cast<float*>(workspace);
+    a.pdl = g_pdl;
+    if (!attention_applies(a)) return MARLIN_Q4_ERR_UNSUPPORTED;
+    return cuda_status(launch_paged_attention(a, static_cast<cudaStream_t>(stream)));
 }
 
 int marlin_q4_rms_norm(const void* x, int32_t x_dtype, const uint16_t* weight, int64_t m, int64_t h, float eps,

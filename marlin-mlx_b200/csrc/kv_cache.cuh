@@ -1,0 +1,101 @@
+// kv_cache.cuh — the paged, quantized key/value cache: its byte layout and the launchers of the
+// operators around it (write, read, head norms with rotation, attention).
+//
+// Pool: [pages][kv_heads][page_size / 16] units.  A unit holds 16 consecutive positions of one head:
+//   [key codes | key scale/bias pairs | value codes | value scale/bias pairs]
+// so one bulk copy brings everything a step of attention over 16 positions reads.  Codes are the
+// group-affine format of the weights (groups of 64 features, value = scale * code + bias, 4-bit
+// codes low nibble first), 4 or 8 bits.  The order of the bytes inside a unit is that of the
+// attention kernel's shared-memory loads, each free of bank conflicts:
+//   key codes    column panels of up to 64 bytes, [panel][row][byte]: a quarter warp (2 rows x 4
+//                column lanes) reads 128 consecutive bytes;
+//   value codes  16-byte pieces, piece c of row r at (c/2) 32 + (r%2 + 2 (r/8)) 8 + (c%2) 4 + (r/2)%4:
+//                the rows 2t (t = 0..3) of two neighbouring pieces are 128 consecutive bytes;
+//   scale/bias   one 32-bit word {scale, bias as bf16} per row and group, [row][group].
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace marlin {
+
+constexpr int kKvRows = 16;  // positions per unit
+
+constexpr int kv_row_bytes(int dim, int bits) { return dim * bits / 8; }
+constexpr int kv_unit_bytes(int dim, int bits) { return kKvRows * 2 * (kv_row_bytes(dim, bits) + 4 * (dim / 64)); }
+
+// Byte offsets inside a unit; rb = row bytes, j = byte within the row's codes, groups = dim / 64.
+__host__ __device__ constexpr int kv_key_code(int r, int j, int rb) {
+    const int p = rb < 64 ? rb : 64;
+    return (j / p) * (p * kKvRows) + r * p + j % p;
+}
+__host__ __device__ constexpr int kv_key_pair(int r, int g, int rb, int groups) {
+    return kKvRows * rb + (r * groups + g) * 4;
+}
+__host__ __device__ constexpr int kv_value_code(int r, int j, int rb, int groups) {
+    const int c = j / 16;
+    return kKvRows * (rb + 4 * groups) + ((c / 2) * 32 + (r % 2 + 2 * (r / 8)) * 8 + (c % 2) * 4 + (r / 2) % 4) * 16 + j % 16;
+}
+__host__ __device__ constexpr int kv_value_pair(int r, int g, int rb, int groups) {
+    return kKvRows * (2 * rb + 4 * groups) + (r * groups + g) * 4;
+}
+
+struct KvPool {
+    uint8_t* data;
+    int64_t pages;
+    int page_units;  // page_size / 16
+    int kv_heads;
+    int dim;
+    int bits;
+};
+
+// k, v: [tokens, kv_heads, dim] of dtype (0 bf16, 1 f32) with token and head strides in elements.
+cudaError_t launch_kv_write(const KvPool& c, const void* k, int64_t k_ts, int64_t k_hs, const void* v, int64_t v_ts,
+                            int64_t v_hs, int dtype, const int32_t* slots, int64_t tokens, bool pdl, cudaStream_t stream);
+cudaError_t launch_kv_read(const KvPool& c, const int32_t* slots, int64_t tokens, uint16_t* k, uint16_t* v, bool pdl,
+                           cudaStream_t stream);
+
+struct RopeArgs {
+    const void* q;
+    const void* k;
+    int64_t q_ts, q_hs, k_ts, k_hs;  // strides in elements
+    int64_t tokens;
+    int heads, kv_heads, dim;
+    const uint16_t* qw;
+    const uint16_t* kw;
+    float eps;
+    const int32_t* positions;  // [axes][tokens]
+    const float* freqs;        // [rot / 2]
+    int rot, interleaved;
+    uint32_t axis[8];          // two bits per frequency
+    void* q_out;
+    void* k_out;
+};
+cudaError_t launch_qk_norm_rope(const RopeArgs& a, int dtype, int out_dtype, bool pdl, cudaStream_t stream);
+
+struct AttnArgs {
+    const uint16_t* q;  // [tokens, heads, dim] bf16, strides in elements
+    int64_t q_ts, q_hs;
+    KvPool pool;
+    int64_t tokens;
+    int heads, group;  // group = heads / kv_heads
+    const int32_t* table;
+    int64_t table_stride;
+    int table_width;
+    const int32_t* kv_lens;
+    const int32_t* cu_q;  // null: one token per sequence
+    int batch, max_q;
+    float scale_log2;     // scale * log2(e)
+    uint16_t* out;        // [tokens, heads, dim]
+    float* part;          // workspace
+    bool pdl;
+};
+constexpr int kAttnMaxBatch = 1024;
+size_t attn_workspace_bytes(int64_t tokens, int heads, int kv_heads, int dim, int batch);
+bool attention_applies(const AttnArgs& a);  // the work's index fits its 32 bits
+cudaError_t launch_paged_attention(const AttnArgs& a, cudaStream_t stream);
+
+int kv_device_error(bool clear);
+int attn_device_error(bool clear);
+
+}  // namespace marlin

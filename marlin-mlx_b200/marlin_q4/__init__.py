@@ -8,7 +8,10 @@ from .ops import (DecodeStep, GreedyLoop, HostDecodeStep, Layer, LmHeadWorkspace
                   device_error, embed_q4, gate_up_swiglu, lm_head_argmax, matmul_residual, mlp_forward,
                   matmul_f32, next_token_after_prefill, qmatmul, quantize_weight, residual_add, rms_norm, set_decode_path,
                   set_pdl, set_step_kernels, decode_step_kernels, synth_bf16)
+from .attention import (KVCache, Rotary, attention_workspace_size, kv_read, kv_write, paged_attention,  # noqa: F401
+                        qk_norm_rope)
 
-__all__ = ["QuantizedTensor", "quantize_weight", "qmatmul", "matmul_f32", "cast_bf16", "rms_norm", "gate_up_swiglu", "matmul_residual",
+__all__ = ["KVCache", "Rotary", "attention_workspace_size", "kv_read", "kv_write", "paged_attention", "qk_norm_rope",
+           "QuantizedTensor", "quantize_weight", "qmatmul", "matmul_f32", "cast_bf16", "rms_norm", "gate_up_swiglu", "matmul_residual",
            "mlp_forward", "residual_add", "lm_head_argmax", "LmHeadWorkspace", "decode_keys", "Layer",
            "DecodeStep", "GreedyLoop", "HostDecodeStep", "embed_q4", "next_token_after_prefill", "synth_bf16", "device_error", "set_pdl", "set_decode_path", "set_step_kernels", "decode_step_kernels", "load", "LIB_PATH", "MarlinQ4Error"]

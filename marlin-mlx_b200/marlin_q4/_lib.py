@@ -33,6 +33,13 @@ class Q4Layer(ctypes.Structure):
                 ("down_proj", Q4Tensor)]
 
 
+class KvCache(ctypes.Structure):
+    """marlin_q4_kv_cache"""
+    _fields_ = [("data", _vp), ("pages", _i64), ("page_size", _i32), ("kv_heads", _i32), ("head_dim", _i32),
+                ("bits", _i32)]
+
+
+_PC = ctypes.POINTER(KvCache)
 _PT, _PL = ctypes.POINTER(Q4Tensor), ctypes.POINTER(Q4Layer)
 
 SIGNATURES = {
@@ -73,6 +80,14 @@ SIGNATURES = {
     "marlin_q4_ipc_open_handle": (ctypes.c_int, [_vp, ctypes.POINTER(ctypes.c_void_p)]),
     "marlin_q4_ipc_close_handle": (ctypes.c_int, [_vp]),
     "marlin_q4_embed": (ctypes.c_int, [_vp, _i64, _PT, _vp, _vp]),
+    "marlin_q4_kv_unit_bytes": (_sz, [_i32, _i32]),
+    "marlin_q4_qk_norm_rope": (ctypes.c_int, [_vp, _i64, _i64, _vp, _i64, _i64, _i32, _i64, _i32, _i32, _i32, _vp, _vp,
+                                              _f32, _vp, _i32, ctypes.c_char_p, _vp, _i32, _i32, _vp, _vp, _i32, _vp]),
+    "marlin_q4_kv_write": (ctypes.c_int, [_PC, _vp, _i64, _i64, _vp, _i64, _i64, _i32, _vp, _i64, _vp]),
+    "marlin_q4_kv_read": (ctypes.c_int, [_PC, _vp, _i64, _vp, _vp, _vp]),
+    "marlin_q4_paged_attention": (ctypes.c_int, [_vp, _i64, _i64, _PC, _i64, _i32, _vp, _i64, _i32, _vp, _vp, _i32,
+                                                 _i32, _f32, _vp, _vp, _sz, _vp]),
+    "marlin_q4_paged_attention_workspace_size": (_sz, [_i64, _i32, _i32, _i32, _i32]),
     "marlin_q4_synth_bf16": (ctypes.c_int, [_vp, _i64, _u64, _f32, _f32, _vp]),
 }
 

@@ -1,0 +1,177 @@
+"""CPU tests of the attention operators' argument checks: every refusal comes before any CUDA call."""
+import ctypes
+
+import pytest
+import torch
+
+import marlin_q4 as mq
+from marlin_q4 import _lib as L
+
+P = 0x100000  # never dereferenced
+
+
+@pytest.fixture(scope="module")
+def lib():
+    return L.load()
+
+
+def cache(data=P, pages=4, page_size=32, kv_heads=2, head_dim=128, bits=4):
+    return L.KvCache(data, pages, page_size, kv_heads, head_dim, bits)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("bits", [4, 8])
+def test_unit_bytes(lib, dim, bits):
+    assert lib.marlin_q4_kv_unit_bytes(dim, bits) == 16 * 2 * (dim * bits // 8 + 4 * dim // 64)
+
+
+@pytest.mark.parametrize("dim,bits", [(32, 4), (96, 4), (512, 8), (128, 2), (128, 16), (0, 4), (-64, 4)])
+def test_unit_bytes_unsupported(lib, dim, bits):
+    assert lib.marlin_q4_kv_unit_bytes(dim, bits) == 0
+
+
+BAD_CACHES = [(dict(data=None), L.ERR_ARG), (dict(pages=0), L.ERR_ARG), (dict(kv_heads=0), L.ERR_ARG),
+              (dict(page_size=0), L.ERR_SHAPE), (dict(page_size=24), L.ERR_SHAPE), (dict(page_size=-16), L.ERR_SHAPE),
+              (dict(page_size=8192), L.ERR_UNSUPPORTED), (dict(head_dim=96), L.ERR_UNSUPPORTED),
+              (dict(bits=16), L.ERR_UNSUPPORTED), (dict(pages=1 << 27), L.ERR_UNSUPPORTED),
+              (dict(data=P + 8), L.ERR_ALIGN)]
+
+
+@pytest.mark.parametrize("bad,status", BAD_CACHES)
+def test_bad_caches(lib, bad, status):
+    c = ctypes.byref(cache(**bad))
+    assert lib.marlin_q4_kv_write(c, P, 256, 128, P, 256, 128, L.BF16, P, 1, None) == status
+    assert lib.marlin_q4_kv_read(c, P, 1, P, P, None) == status
+    assert lib.marlin_q4_paged_attention(P, 512, 128, c, 1, 4, P, 1, 1, P, None, 1, 1, 0.1, P, P, 1 << 40, None) == status
+
+
+def test_write_and_read(lib):
+    c = ctypes.byref(cache())
+    write, read = lib.marlin_q4_kv_write, lib.marlin_q4_kv_read
+    assert write(c, None, 256, 128, P, 256, 128, L.BF16, P, 1, None) == L.ERR_ARG
+    assert write(c, P, 256, 128, None, 256, 128, L.BF16, P, 1, None) == L.ERR_ARG
+    assert write(c, P, 256, 128, P, 256, 128, 5, P, 1, None) == L.ERR_ARG
+    assert write(c, P, 256, 128, P, 256, 128, L.BF16, None, 1, None) == L.ERR_ARG
+    assert write(c, P, 256, 128, P, 256, 128, L.BF16, P, -1, None) == L.ERR_ARG
+    assert write(c, P, -256, 128, P, 256, 128, L.BF16, P, 1, None) == L.ERR_ARG
+    assert write(c, P + 2, 256, 128, P, 256, 128, L.BF16, P, 1, None) == L.ERR_ALIGN
+    assert write(c, P, 260, 128, P, 256, 128, L.BF16, P, 1, None) == L.ERR_ALIGN
+    assert write(c, P, 256, 128, P, 256, 130, L.F32, P, 1, None) == L.ERR_ALIGN
+    assert write(c, P, 256, 128, P, 256, 128, L.BF16, P + 2, 1, None) == L.ERR_ALIGN
+    assert write(c, P, 256, 128, P, 256, 128, L.BF16, P, 1 << 25, None) == L.ERR_UNSUPPORTED
+    assert write(c, P, 256, 128, P, 256, 128, L.BF16, P, 0, None) == L.OK
+    assert read(c, None, 1, P, P, None) == L.ERR_ARG
+    assert read(c, P, 1, None, P, None) == L.ERR_ARG
+    assert read(c, P, 1, P, P + 8, None) == L.ERR_ALIGN
+    assert read(c, P, 1 << 25, P, P, None) == L.ERR_UNSUPPORTED
+    assert read(c, P, 0, None, None, None) == L.OK
+
+
+def rope(lib, **kw):
+    a = dict(q=P, qt=1024, qh=128, k=P, kt=256, kh=128, dtype=L.BF16, tokens=3, heads=8, kv_heads=2, dim=128, qw=P, kw=P,
+             eps=1e-6, positions=P, axes=1, axis_of=None, freqs=P, rot=64, interleaved=0, qo=P, ko=P, out=L.BF16)
+    a.update(kw)
+    return lib.marlin_q4_qk_norm_rope(*a.values(), None)
+
+
+@pytest.mark.parametrize("bad,status", [
+    (dict(q=None), L.ERR_ARG), (dict(k=None), L.ERR_ARG), (dict(dtype=3), L.ERR_ARG), (dict(out=-1), L.ERR_ARG),
+    (dict(tokens=-1), L.ERR_ARG), (dict(heads=0), L.ERR_ARG), (dict(kv_heads=0), L.ERR_ARG), (dict(axes=0), L.ERR_ARG),
+    (dict(axes=5), L.ERR_ARG), (dict(qw=None), L.ERR_ARG), (dict(positions=None), L.ERR_ARG), (dict(freqs=None), L.ERR_ARG),
+    (dict(qo=None), L.ERR_ARG), (dict(axes=2, axis_of=b"\0" * 31 + b"\2"), L.ERR_ARG), (dict(dim=80), L.ERR_UNSUPPORTED),
+    (dict(rot=0), L.ERR_SHAPE), (dict(rot=24), L.ERR_SHAPE), (dict(rot=144), L.ERR_SHAPE),
+    (dict(tokens=1 << 25), L.ERR_UNSUPPORTED), (dict(heads=2000), L.ERR_UNSUPPORTED), (dict(q=P + 2), L.ERR_ALIGN),
+    (dict(qt=1025), L.ERR_ALIGN), (dict(kh=132), L.ERR_ALIGN), (dict(kw=P + 4), L.ERR_ALIGN), (dict(ko=P + 2), L.ERR_ALIGN)])
+def test_rope_refusals(lib, bad, status):
+    assert rope(lib, **bad) == status
+
+
+def test_rope_of_nothing(lib):
+    assert rope(lib, tokens=0) == L.OK
+
+
+def attend(lib, **kw):
+    a = dict(q=P, qt=512, qh=128, cache=cache(), tokens=3, heads=4, table=P, ts=2, tw=2, lens=P, cu=None, batch=3, max_q=1,
+             scale=0.1, out=P, ws=P, wsb=1 << 40)
+    a.update(kw)
+    a["cache"] = ctypes.byref(a["cache"])
+    return lib.marlin_q4_paged_attention(*a.values(), None)
+
+
+@pytest.mark.parametrize("bad,status", [
+    (dict(q=None), L.ERR_ARG), (dict(table=None), L.ERR_ARG), (dict(lens=None), L.ERR_ARG), (dict(out=None), L.ERR_ARG),
+    (dict(tokens=-1), L.ERR_ARG), (dict(heads=0), L.ERR_ARG), (dict(batch=-1), L.ERR_ARG), (dict(tw=-1), L.ERR_ARG),
+    (dict(scale=0.0), L.ERR_ARG), (dict(scale=-0.1), L.ERR_ARG), (dict(scale=float("nan")), L.ERR_ARG),
+    (dict(scale=float("inf")), L.ERR_ARG), (dict(cu=P, max_q=-1), L.ERR_ARG), (dict(heads=5), L.ERR_SHAPE),
+    (dict(batch=2), L.ERR_SHAPE), (dict(tokens=1025, batch=1025), L.ERR_UNSUPPORTED),
+    (dict(tokens=1 << 25, cu=P), L.ERR_UNSUPPORTED), (dict(tw=1 << 30), L.ERR_UNSUPPORTED), (dict(q=P + 8), L.ERR_ALIGN),
+    (dict(qt=516), L.ERR_ALIGN), (dict(out=P + 2), L.ERR_ALIGN), (dict(table=P + 2), L.ERR_ALIGN),
+    (dict(ws=None), L.ERR_WORKSPACE), (dict(ws=P + 16), L.ERR_WORKSPACE), (dict(wsb=64), L.ERR_WORKSPACE)])
+def test_attention_refusals(lib, bad, status):
+    assert attend(lib, **bad) == status
+
+
+def test_attention_of_nothing(lib):
+    assert attend(lib, tokens=0, batch=0) == L.OK
+    assert attend(lib, tokens=5, batch=0, cu=P) == L.OK
+    assert attend(lib, tokens=5, cu=P, max_q=0) == L.OK
+
+
+def test_workspace_size(lib):
+    size = lib.marlin_q4_paged_attention_workspace_size
+    assert size(1, 8, 2, 256, 1) > 0
+    for bad in ((-1, 8, 2, 256, 1), (1, 0, 2, 256, 1), (1, 8, 3, 256, 1), (1, 8, 2, 80, 1), (1, 8, 2, 256, 0), (1, 8, 2, 256, 4096)):
+        assert size(*bad) == 0
+    with pytest.raises(ValueError):
+        mq.attention_workspace_size(1, 8, 3, 256, 1)
+
+
+def test_front_end_refusals():
+    z = torch.zeros
+    data = z((2, 2, 1, 16 * 2 * (64 + 8)), dtype=torch.uint8)
+    c = mq.KVCache(data, 128, 4)
+    assert (c.pages, c.page_size, c.kv_heads) == (2, 16, 2)
+    with pytest.raises(ValueError):
+        mq.KVCache(data, 128, 8)
+    with pytest.raises(ValueError):
+        mq.KVCache(data, 96, 4)
+    with pytest.raises(ValueError):
+        mq.KVCache(data.transpose(0, 1), 128, 4)
+    with pytest.raises(ValueError):
+        mq.KVCache.empty(2, 20, 2, 128, device="cpu")
+    k = z((3, 2, 128), dtype=torch.bfloat16)
+    slots = z(3, dtype=torch.int32)
+    with pytest.raises(ValueError):  # CPU tensors
+        mq.kv_write(c, k, k, slots)
+    with pytest.raises(ValueError):
+        mq.kv_read(c, slots)
+    with pytest.raises(TypeError):
+        mq.kv_write(c, k.half(), k.half(), slots)
+    with pytest.raises(TypeError):
+        mq.kv_write(c, k, k, slots.long())
+    with pytest.raises(ValueError):
+        mq.kv_write(c, k[:, :1], k[:, :1], slots)
+    with pytest.raises(ValueError):
+        mq.kv_write(c, k, k, slots[:2])
+    with pytest.raises(ValueError):
+        mq.Rotary(z(32, dtype=torch.float64))
+    with pytest.raises(ValueError):
+        mq.Rotary(z(32), axes=[0] * 31)
+    q = z((3, 4, 128), dtype=torch.bfloat16)
+    w = z(128, dtype=torch.bfloat16)
+    rot = mq.Rotary(z(32))
+    with pytest.raises(ValueError):
+        mq.qk_norm_rope(q, k, w, w, slots, rot)
+    with pytest.raises(TypeError):
+        mq.qk_norm_rope(q, k.float(), w, w, slots, rot)
+    with pytest.raises(ValueError):
+        mq.qk_norm_rope(q, k, w[:64], w, slots, rot)
+    table = z((3, 2), dtype=torch.int32)
+    with pytest.raises(ValueError):
+        mq.paged_attention(q, c, table, slots)
+    with pytest.raises(TypeError):
+        mq.paged_attention(q.float(), c, table, slots)
+    with pytest.raises(ValueError):
+        mq.paged_attention(q[..., :64], c, table, slots)
+    with pytest.raises(ValueError):
+        mq.paged_attention(q, c, table.long(), slots)
