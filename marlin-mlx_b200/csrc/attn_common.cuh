@@ -12,36 +12,31 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
-// bf16x2 of (lo, hi), each rounded to nearest even
+// bf16x2 / f16x2 of (lo, hi), each rounded to nearest even
 __device__ __forceinline__ uint32_t bf16x2_of(float lo, float hi) {
     uint32_t d;
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
     return d;
 }
-
-__device__ __forceinline__ uint32_t bf16x2_min(uint32_t a, uint32_t b) {
+__device__ __forceinline__ uint32_t f16x2_of(float lo, float hi) {
     uint32_t d;
-    asm("min.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+    return d;
+}
+__device__ __forceinline__ uint32_t f16x2_add(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("add.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
     return d;
 }
 
-constexpr uint32_t kBf16One2 = 0x3F803F80u, kBf16Neg128x2 = 0xC300C300u, kBf16Half2 = 0x3F003F00u,
-                   kBf16Magic = 0x43004300u, kBf16NegZero2 = 0x80008000u;
+// f16 keeps 10 fraction bits: OR-ing the exponent of 1024 onto an integer below 1024 gives 1024 + it,
+// exactly.  A code at bits [0, 4) becomes 1024 + q, one left at bits [4, 8) becomes 1024 + 16 q without
+// a shift; an 8-bit code takes the upper byte of the constant by a byte permute.
+constexpr uint32_t kF16Magic = 0x64006400u, kF16MagicBytes = 0x64646464u;
+constexpr uint32_t kF16Neg1032x2 = 0xE408E408u, kF16Neg1152x2 = 0xE480E480u;  // -(1024 + 8), -(1024 + 128)
 
-// Two 4-bit codes at bits [0,4) and [16,20) of w -> bf16x2 s q + b.  OR-ing the exponent of 128 gives
-// 128 + q exactly, one FMA removes the 128 (exact), one forms q s + b with a single rounding.
-__device__ __forceinline__ uint32_t dequant4(uint32_t w, uint32_t s2, uint32_t b2) {
-    const uint32_t v = lop3_and_or(w, 0x000F000Fu, kBf16Magic);
-    return bf16x2_fma(bf16x2_fma(v, kBf16One2, kBf16Neg128x2), s2, b2);
-}
-// Two 8-bit codes at bits [0,8) and [16,24) of w -> bf16x2 s q + b.  bf16 keeps 7 fraction bits, so the
-// OR gives v = 128 + q below 128 and v = 2 q from 128 on (bit 7 lands on the exponent): q is the smaller
-// of v - 128 and v / 2 in both cases, every step exact.
-__device__ __forceinline__ uint32_t dequant8(uint32_t w, uint32_t s2, uint32_t b2) {
-    const uint32_t v = lop3_and_or(w, 0x00FF00FFu, kBf16Magic);
-    const uint32_t q = bf16x2_min(bf16x2_fma(v, kBf16One2, kBf16Neg128x2), bf16x2_fma(v, kBf16Half2, kBf16NegZero2));
-    return bf16x2_fma(q, s2, b2);
-}
+// The power of two 2^e as binary32, e in [-126, 127]
+__device__ __forceinline__ float pow2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
 // The tokens [q0, q0 + n) and cached positions of sequence b, made safe: starts clamped to the tokens,
 // at most max_q of them, lengths clamped to what the table can hold.  What had to be cut is recorded.

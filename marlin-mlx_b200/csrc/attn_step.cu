@@ -1,20 +1,27 @@
 // attn_step.cu — attention of few query rows over the paged, quantized cache: decode steps and short
-// runs of new tokens.
+// runs of new tokens (at most 16 (token, head of the group) rows per kv head).
 //
-// Rows are the (token, head of the group) pairs of one kv head, 8 or 16 to a tile.  Per tile and 16
-// cached positions, with K and V dequantized in registers (bf16, one rounding of the exact value):
-//   S^T[16 x rows] = K Q^T          mma m16n8k16, A = K from the codes, B = Q
-//   P = 2^(S scale log2e - m)       running maximum m and sum l per row, binary32
-//   O^T[dim x rows] += V^T P^T      A = V^T from the codes, B = P^T (one 8x8 transpose of the bf16 pairs)
-// Taking the positions (then the features) as the M side lets 8 rows fill an MMA, so a decode step of
-// up to 8 heads per kv head wastes none of the dequantized operand.
+// Per tile of 8 or 16 rows and unit of 16 cached positions, with f16 tensor-core MMAs (m16n8k16, sums in
+// binary32) whose cache operand is made of the raw codes:
+//   S^T[16 x rows] = K Q^T     per 64-feature group g:  acc = sum q (1024 + code), started at -1024 sum q,
+//                              S += s_kg acc + b_kg sum q: keys are never rounded;
+//   p = 2^(S scale log2e - M)  running maximum and sum per row, binary32;
+//   O^T[dim x rows] += V^T P^T A = code - 8 (or - 128), exact; B = p s_kg rounded to f16 (11 bits);
+//                              the rest of the value, sum p (b_kg + 8 s_kg), is summed in binary32.
+// Codes reach f16 by OR-ing an exponent (see attn_common.cuh), one instruction per two values (a nibble
+// left in place counts 16-fold, which the query fragment or the final row undoes).  f16 ranges: the
+// queries of a row are scaled by a power of two to a maximum in [2^12, 2^13); M is the running maximum of
+// (S + e), e the exponent of the largest value scale in the pair of units, so that p s stays below 2
+// whatever the values' size.
+// Taking the positions (then the features) as the M side lets 8 rows fill an MMA, so a decode step of up
+// to 8 heads per kv head wastes none of the cache operand.
 //
-// Bound: bytes of the cache, or the issue slots of the dequantization (about 2 instructions per value
-// at 4 bits).  Each warp owns a ring of units fed by bulk copies (one contiguous unit per copy) and
-// takes every fourth pair of units of its CTA's range, with its own m, l and O; the four warps are
-// joined once at the end of a range in shared memory.  The work of all tiles, in units, is laid end to
-// end and cut into equal shares, one per CTA, so that lengths of any mix load the SMs evenly; a tile
-// that several CTAs touched is joined by a second kernel from their partial rows, in a fixed order.
+// Bound: bytes of the cache or issue slots (about 1.2 instructions per cached value).  Each warp owns a
+// ring of units fed by bulk copies (one contiguous unit per copy) and takes every fourth pair of units of
+// its CTA's range, with its own M, sums and O; the four warps are joined once at the end of a range in
+// shared memory.  The tiles' work, in units plus kTileCost for a tile's fixed cost, is laid end to end
+// and cut into equal shares, one per CTA, so that lengths of any mix load the SMs evenly; a tile that
+// several CTAs touched is joined by a second kernel from their partial rows, in a fixed order.
 #include <algorithm>
 
 #include "attn_common.cuh"
@@ -25,26 +32,27 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr int kMinShare = 2 * kWarps;  // units: one pair per warp
+constexpr uint32_t kTileCost = 8;    // fixed cost of a tile (queries, joining the warps), in units
+constexpr uint32_t kMinShare = kTileCost + 2 * kWarps;  // units: one pair per warp
 
 template <int D, int BITS, int NT>
 struct StepCfg {
     static constexpr int RB = kv_row_bytes(D, BITS), G = D / 64, UB = kv_unit_bytes(D, BITS);
     static constexpr int ROWS = 8 * NT;
-    static constexpr int STEPS = D / 16;   // MMAs along the features
-    static constexpr int PANELS = RB < 64 ? 1 : RB / 64;
-    static constexpr int CTAS = NT == 2 ? (D == 256 ? 1 : D == 128 ? 2 : 4) : D == 256 ? (BITS == 4 ? 3 : 2) : D == 128 ? (BITS == 4 ? 4 : 3) : 5;
+    static constexpr int CTAS = NT == 2 ? (D == 256 ? 1 : D == 128 ? 3 : 4) : D == 256 ? (BITS == 4 ? 3 : 2) : D == 128 ? (BITS == 4 ? 4 : 3) : 5;
     static constexpr int RING = D == 256 ? 3 : D == 128 ? (BITS == 4 ? 4 : 3) : (BITS == 4 ? 6 : 4);
     static constexpr uint32_t RING_BYTES = kWarps * RING * UB;
     static constexpr uint32_t MERGE_BYTES = kWarps * ROWS * D * 4;
     static constexpr uint32_t OFF_Q = RING_BYTES > MERGE_BYTES ? RING_BYTES : MERGE_BYTES;
-    static constexpr uint32_t OFF_ML = OFF_Q + NT * STEPS * 32 * 8;
+    static constexpr uint32_t OFF_SUM = OFF_Q + NT * G * 4 * 32 * 8;  // query fragments [NT][G][4][32]
+    static constexpr uint32_t OFF_SR = OFF_SUM + ROWS * G * 8;        // query sums [NT][G][4 lanes][2 rows]
+    static constexpr uint32_t OFF_ML = OFF_SR + ROWS * 4;             // score factor per row
     static constexpr uint32_t OFF_BAR = OFF_ML + kWarps * ROWS * 8;
     static constexpr uint32_t OFF_PRE = OFF_BAR + kWarps * RING * 8;
-    static constexpr uint32_t SMEM = OFF_PRE + (kAttnMaxBatch + 1) * 4 + 64;
+    static constexpr uint32_t SMEM = OFF_PRE + (kAttnMaxBatch + 1) * 4;
 };
 
-// Workspace: [kAttnMaxBatch + 1] u32 prefix of the work, share (u32), then per slot ROWS (m, l) pairs,
+// Workspace: [kAttnMaxBatch + 1] u32 prefix of the work, share (u32), then per slot ROWS (M, l) pairs,
 // then per slot [ROWS][D] partial rows.  Slots 2 c and 2 c + 1 belong to CTA c (its first range, its last).
 struct StepWork {
     uint32_t* prefix;
@@ -61,23 +69,52 @@ __host__ __device__ inline StepWork step_work(float* part, int grid, int rows) {
     return w;
 }
 
-__device__ __forceinline__ uint32_t seq_work(const AttnArgs& a, const SeqSpan& s, int rows) {
-    const uint32_t tiles = (uint32_t)((s.n * a.group + rows - 1) / rows);
-    return (uint32_t)a.pool.kv_heads * tiles * (uint32_t)((s.len + kKvRows - 1) / kKvRows);
+__device__ __forceinline__ uint32_t units_of(int len) { return (uint32_t)((len + kKvRows - 1) / kKvRows); }
+// one tile per (sequence with new tokens and positions, kv head)
+__device__ __forceinline__ uint32_t tile_work(const SeqSpan& s) {
+    return s.n > 0 && s.len > 0 ? units_of(s.len) + kTileCost : 0u;
 }
 
 __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
     uint32_t y;
-    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
+
+// D += A B, f16 operands, binary32 sums; fragment layout of mma_bf16_16816
+__device__ __forceinline__ void mma_f16_16816(float d[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                              uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
+        "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+template <int G>
+__device__ __forceinline__ void load_pairs(const uint8_t* p, uint32_t (&w)[G]) {
+    if constexpr (G == 4) {
+        const uint4 x = lds128(p);
+        w[0] = x.x, w[1] = x.y, w[2] = x.z, w[3] = x.w;
+    } else if constexpr (G == 2) {
+        const uint2 x = lds64(p);
+        w[0] = x.x, w[1] = x.y;
+    } else {
+        w[0] = *reinterpret_cast<const uint32_t*>(p);
+    }
+}
+__device__ __forceinline__ float pair_scale(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float pair_bias(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
 
 template <int D, int BITS, int NT>
 __global__ void __launch_bounds__(kThreads, StepCfg<D, BITS, NT>::CTAS) attn_step_kernel(const __grid_constant__ AttnArgs a) {
     using C = StepCfg<D, BITS, NT>;
+    constexpr int G = C::G;
     extern __shared__ __align__(128) uint8_t smem[];
     uint32_t* pre = reinterpret_cast<uint32_t*>(smem + C::OFF_PRE);
-    uint2* qf = reinterpret_cast<uint2*>(smem + C::OFF_Q);       // [NT][STEPS][32]
+    uint2* qf = reinterpret_cast<uint2*>(smem + C::OFF_Q);
+    float2* qsum = reinterpret_cast<float2*>(smem + C::OFF_SUM);
+    float* qsr = reinterpret_cast<float*>(smem + C::OFF_SR);
     float2* ml = reinterpret_cast<float2*>(smem + C::OFF_ML);    // [warp][ROWS]
     float4* merge = reinterpret_cast<float4*>(smem);             // [warp][ROWS][D / 4], over the ring
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
@@ -93,7 +130,7 @@ __global__ void __launch_bounds__(kThreads, StepCfg<D, BITS, NT>::CTAS) attn_ste
     }
     pdl_wait();
     pdl_launch_dependents();
-    // prefix sums of the sequences' work, in units
+    // prefix sums of the sequences' work
     uint32_t base = 0;
     if (tid == 0) pre[0] = 0;
     for (int b0 = 0; b0 < a.batch; b0 += kThreads) {
@@ -101,7 +138,7 @@ __global__ void __launch_bounds__(kThreads, StepCfg<D, BITS, NT>::CTAS) attn_ste
         uint32_t v = 0;
         if (b < a.batch) {
             const SeqSpan s = seq_span(a, b);
-            v = seq_work(a, s, C::ROWS);
+            v = tile_work(s) * (uint32_t)a.pool.kv_heads;
             if (s.len == 0 && b % gridDim.x == blockIdx.x)  // no position to attend to: zero rows
                 for (int64_t i = 0; i < (int64_t)s.n * a.heads * D / 8; ++i)
                     reinterpret_cast<uint4*>(a.out + (int64_t)s.q0 * a.heads * D)[i] = make_uint4(0u, 0u, 0u, 0u);
@@ -112,7 +149,7 @@ __global__ void __launch_bounds__(kThreads, StepCfg<D, BITS, NT>::CTAS) attn_ste
             const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
             if (lane >= o) x += y;
         }
-        __syncthreads();
+        if (b0) __syncthreads();
         if (lane == 31) wsum[warp] = x;
         __syncthreads();
         uint32_t before = base, all = base;
@@ -126,7 +163,7 @@ __global__ void __launch_bounds__(kThreads, StepCfg<D, BITS, NT>::CTAS) attn_ste
     }
     __syncthreads();
     const uint32_t total = base;
-    const uint32_t share = max((uint32_t)kMinShare, (total + gridDim.x - 1) / gridDim.x);
+    const uint32_t share = max(kMinShare, (total + gridDim.x - 1) / gridDim.x);
     const StepWork work = step_work(a.part, gridDim.x, C::ROWS);
     if (blockIdx.x == 0) {
         for (int b = tid; b <= a.batch; b += kThreads) work.prefix[b] = pre[b];
@@ -137,7 +174,7 @@ __global__ void __launch_bounds__(kThreads, StepCfg<D, BITS, NT>::CTAS) attn_ste
 
     uint32_t done = 0;  // units this warp has consumed so far (ring position and phase)
     for (uint32_t w0 = (uint32_t)min(w_begin, (uint64_t)total); w0 < w_end;) {
-        // the range's sequence, kv head, row tile and units
+        // the range's sequence, kv head and units; a tile's first kTileCost steps carry no units
         int lo = 0, hi = a.batch - 1;
         while (lo < hi) {
             const int mid = (lo + hi + 1) >> 1;
@@ -145,37 +182,38 @@ __global__ void __launch_bounds__(kThreads, StepCfg<D, BITS, NT>::CTAS) attn_ste
         }
         const int b = lo;
         const SeqSpan s = seq_span(a, b);
-        const uint32_t nu = (uint32_t)((s.len + kKvRows - 1) / kKvRows);
-        const uint32_t tiles = (uint32_t)((s.n * a.group + C::ROWS - 1) / C::ROWS);
-        const uint32_t in = w0 - pre[b], ti = in / nu;
-        const int u0 = (int)(in - ti * nu), h = (int)(ti / tiles), row0 = (int)(ti % tiles) * C::ROWS;
-        const int u1 = (int)min((uint32_t)nu, (uint32_t)u0 + (w_end - w0));
+        const uint32_t nu = units_of(s.len), vl = nu + kTileCost;
+        const uint32_t in = w0 - pre[b];
+        const int h = (int)(in / vl);
+        const uint32_t v0 = in - h * vl, v1 = min(vl, v0 + (w_end - w0));
+        const int u0 = (int)(max(v0, kTileCost) - kTileCost), u1 = (int)(max(v1, kTileCost) - kTileCost);
         const bool whole = u0 == 0 && u1 == (int)nu;
         const int slot = 2 * (int)blockIdx.x + (w0 == (uint32_t)w_begin ? 0 : 1);
-        w0 += (uint32_t)(u1 - u0);
-        const int nrows = min(C::ROWS, s.n * a.group - row0);
+        w0 += v1 - v0;
+        if (u0 >= u1) continue;
+        const int nrows = s.n * a.group;  // at most ROWS
         // row r sees the positions below len - n + token + 1
-        const int last_seen = s.len - s.n + (row0 + nrows - 1) / a.group + 1;
-        const int first_seen = s.len - s.n + row0 / a.group + 1;
-        const int ue = min(u1, (max(last_seen, 0) + kKvRows - 1) / kKvRows);  // units beyond hold nothing seen
+        const int first_seen = min(s.len, s.len - s.n + 1);
 
-        // this warp's units: pairs warp, warp + 4, ... of [u0, ue)
+        // this warp's units: pairs warp, warp + 4, ... of [u0, u1)
         auto unit_of = [&](int k) { return u0 + 2 * (warp + kWarps * (k >> 1)) + (k & 1); };
-        const int left = max(0, ue - u0);
+        const int left = u1 - u0;
         const int full = left / (2 * kWarps), rest = left % (2 * kWarps) - 2 * warp;
         const int mine = 2 * full + min(2, max(0, rest));
-        int page = 0, issued = 0;
+        int issued = 0;
+        const uint8_t* src = nullptr;
         auto issue = [&](int upto) {
             for (; issued < upto; ++issued) {
-                if ((issued & 31) == 0) {  // the pages of the next 32 units, one per lane
+                if ((issued & 31) == 0) {  // where the next 32 units stand, one per lane
                     const int k = issued + lane;
-                    if (k < mine) page = table_page(a, b, unit_of(k) / a.pool.page_units);
+                    if (k < mine) {
+                        const int u = unit_of(k), page = u / a.pool.page_units;
+                        src = a.pool.data + (((int64_t)table_page(a, b, page) * a.pool.kv_heads + h) * a.pool.page_units +
+                                             (u - page * a.pool.page_units)) * (int64_t)C::UB;
+                    }
                 }
-                const int64_t pg = __shfl_sync(0xffffffffu, page, issued & 31);
-                if (lane == 0) {
-                    const int u = unit_of(issued);
+                if (lane == (issued & 31)) {
                     const uint32_t at = (done + issued) % C::RING;
-                    const uint8_t* src = a.pool.data + ((pg * a.pool.kv_heads + h) * a.pool.page_units + u % a.pool.page_units) * (int64_t)C::UB;
                     mbar_arrive_expect_tx(&bars[at], C::UB);
                     tma_bulk_g2s(ring + at * C::UB, src, C::UB, &bars[at]);
                 }
@@ -183,47 +221,78 @@ __global__ void __launch_bounds__(kThreads, StepCfg<D, BITS, NT>::CTAS) attn_ste
         };
         issue(min(mine, C::RING));
 
-        // Q as B fragments; feature order = the order in which the key codes unpack
-        for (int i = tid; i < NT * C::STEPS * 32; i += kThreads) {
-            const int ln = i & 31, st = (i >> 5) % C::STEPS, nt = (i >> 5) / C::STEPS;
-            const int r = row0 + nt * 8 + (ln >> 2), tt = ln & 3;
-            uint2 v = make_uint2(0u, 0u);
-            if (nt * 8 + (ln >> 2) < nrows) {
-                const uint16_t* q = a.q + (int64_t)(s.q0 + r / a.group) * a.q_ts + (int64_t)(h * a.group + r % a.group) * a.q_hs;
-                if (BITS == 4) {
-                    const int d = (C::RB < 64 ? tt * 16 + (st >> 1) * 8 : (st >> 3) * 128 + tt * 32 + ((st & 7) >> 1) * 8) + (st & 1) * 2;
-                    v.x = q[d] | ((uint32_t)q[d + 4] << 16);
-                    v.y = q[d + 1] | ((uint32_t)q[d + 5] << 16);
-                } else {
-                    const int d = (st >> 2) * 64 + tt * 16 + (st & 3) * 4;
-                    v.x = q[d] | ((uint32_t)q[d + 2] << 16);
-                    v.y = q[d + 1] | ((uint32_t)q[d + 3] << 16);
-                }
+        // Queries as f16 B fragments, a warp per row: scaled by a power of two to a maximum in [2^12, 2^13),
+        // features in the order in which the key codes unpack; per group sum q and 1024 sum q (1 or 1/16).
+        for (int r = warp; r < C::ROWS; r += kWarps) {
+            constexpr int E = D / 32;
+            float q[E];
+            uint32_t big = 0;
+            const int rr = min(r, nrows - 1);
+            const uint16_t* src_q = a.q + (int64_t)(s.q0 + rr / a.group) * a.q_ts + (int64_t)(h * a.group + rr % a.group) * a.q_hs + lane * E;
+            uint32_t raw[E / 2];
+#pragma unroll
+            for (int i = 0; i < E / 2; ++i) raw[i] = reinterpret_cast<const uint32_t*>(src_q)[i];
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                q[i] = r < nrows ? bf16_bits_to_f32(i & 1 ? raw[i / 2] >> 16 : raw[i / 2] & 0xffffu) : 0.f;
+                big = max(big, __float_as_uint(q[i]) & 0x7fffffffu);
             }
-            qf[i] = v;
+            big = __reduce_max_sync(0xffffffffu, big);
+            const int ex = max((int)(big >> 23) - 127, -100);
+            const float f = pow2i(12 - ex);
+            float sum = 0.f, off = 0.f;
+            uint16_t* qh = reinterpret_cast<uint16_t*>(qf);
+#pragma unroll
+            for (int i = 0; i < E; ++i) {
+                const int d = lane * E + i, grp = d >> 6, tt = (d >> 4) & 3, n = d & 15;
+                const float x = q[i] * f;
+                int st, reg, half;
+                float y = x;
+                if (BITS == 4) {  // word n / 8: nibble pairs (j, j + 4), odd j left in place (16-fold)
+                    st = (n >> 3) * 2 + ((n >> 1) & 1), reg = n & 1, half = (n >> 2) & 1;
+                    if (n & 1) y = x * 0.0625f;
+                } else {
+                    st = n >> 2, reg = (n >> 1) & 1, half = n & 1;
+                }
+                const uint16_t bits = (uint16_t)f16x2_of(y, 0.f);
+                qh[((((r >> 3) * G + grp) * 4 + st) * 32 + (r & 7) * 4 + tt) * 4 + reg * 2 + half] = bits;
+                sum += x;
+                off += y;
+            }
+#pragma unroll
+            for (int o = 1; o < 64 / E; o <<= 1) {
+                sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                off += __shfl_xor_sync(0xffffffffu, off, o);
+            }
+            if (lane % (64 / E) == 0)
+                qsum[(((r >> 3) * G + lane * E / 64) * 4 + ((r & 7) >> 1)) * 2 + (r & 1)] = make_float2(sum, -1024.f * off);
+            if (lane == 0) qsr[r] = a.scale_log2 * pow2i(ex - 12);
         }
         __syncthreads();
 
-        float m[NT][2], l[NT][2], o[NT][D / 16][4];
+        float m[NT][2], l[NT][2], sr[NT][2], o[NT][D / 16][4], bs[NT][G][2];
         int lim[NT][2];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
                 m[nt][x] = -INFINITY;
                 l[nt][x] = 0.f;
-                lim[nt][x] = min(s.len, s.len - s.n + (row0 + nt * 8 + 2 * t + x) / a.group + 1);
-            }
+                sr[nt][x] = qsr[nt * 8 + 2 * t + x];
+                lim[nt][x] = min(s.len, s.len - s.n + (nt * 8 + 2 * t + x) / a.group + 1);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+                for (int gr = 0; gr < G; ++gr) bs[nt][gr][x] = 0.f;
+            }
 #pragma unroll
             for (int j = 0; j < D / 16; ++j)
 #pragma unroll
                 for (int x = 0; x < 4; ++x) o[nt][j][x] = 0.f;
+        }
 
         bool ok = true;
         for (int k = 0; k < mine; k += 2) {
             const bool two = k + 1 < mine;
+            const int pos = unit_of(k) * kKvRows;
             float sc[2][NT][4];
             const uint8_t* up[2];
 #pragma unroll
@@ -237,65 +306,82 @@ __global__ void __launch_bounds__(kThreads, StepCfg<D, BITS, NT>::CTAS) attn_ste
                 if (e == 1 && !two) continue;
                 ok = ok && mbar_wait(&bars[at], ((done + k + e) / C::RING) & 1);
                 const uint8_t* u = up[e];
+                uint32_t p0[G], p1[G];
+                load_pairs<G>(u + kv_key_pair(g, 0, C::RB, G), p0);
+                load_pairs<G>(u + kv_key_pair(g + 8, 0, C::RB, G), p1);
 #pragma unroll
-                for (int p = 0; p < C::PANELS; ++p) {
-                    const int grp = BITS == 4 ? (C::RB < 64 ? 0 : (p * 128 + t * 32) / 64) : p;
-                    const uint32_t k0 = *reinterpret_cast<const uint32_t*>(u + kv_key_pair(g, grp, C::RB, C::G));
-                    const uint32_t k1 = *reinterpret_cast<const uint32_t*>(u + kv_key_pair(g + 8, grp, C::RB, C::G));
-                    const uint32_t s0 = __byte_perm(k0, 0, 0x1010), b0 = __byte_perm(k0, 0, 0x3232);
-                    const uint32_t s1 = __byte_perm(k1, 0, 0x1010), b1 = __byte_perm(k1, 0, 0x3232);
-                    uint32_t w0v[4], w1v[4];
-                    constexpr int NWK = C::RB < 64 ? 2 : 4;
-                    if (C::RB < 64) {
-                        const uint2 x0 = lds64(u + g * 32 + t * 8), x1 = lds64(u + (g + 8) * 32 + t * 8);
-                        w0v[0] = x0.x, w0v[1] = x0.y, w1v[0] = x1.x, w1v[1] = x1.y;
-                    } else {
-                        const uint4 x0 = lds128(u + p * 1024 + g * 64 + t * 16), x1 = lds128(u + p * 1024 + (g + 8) * 64 + t * 16);
-                        w0v[0] = x0.x, w0v[1] = x0.y, w0v[2] = x0.z, w0v[3] = x0.w;
-                        w1v[0] = x1.x, w1v[1] = x1.y, w1v[2] = x1.z, w1v[3] = x1.w;
-                    }
+                for (int gr = 0; gr < G; ++gr) {
+                    // sixteen features of rows g and g + 8 as A fragments of four steps
+                    uint32_t f0[8], f1[8];
+                    if (BITS == 4) {
+                        const uint8_t* at0 = C::RB < 64 ? u + t * 8 : u + (gr >> 1) * 1024 + (gr & 1) * 32 + t * 8;
+                        constexpr int RS = C::RB < 64 ? 32 : 64;
+                        const uint2 x = lds64(at0 + g * RS), y = lds64(at0 + (g + 8) * RS);
+                        const uint32_t xs[2] = {x.x, x.y}, ys[2] = {y.x, y.y};
 #pragma unroll
-                    for (int w = 0; w < NWK; ++w) {
-                        if (BITS == 4) {
-#pragma unroll
-                            for (int hf = 0; hf < 2; ++hf) {
-                                const int st = (p * NWK + w) * 2 + hf;
-                                const uint32_t a0 = dequant4(w0v[w] >> (8 * hf), s0, b0), a2 = dequant4(w0v[w] >> (8 * hf + 4), s0, b0);
-                                const uint32_t a1 = dequant4(w1v[w] >> (8 * hf), s1, b1), a3 = dequant4(w1v[w] >> (8 * hf + 4), s1, b1);
-#pragma unroll
-                                for (int nt = 0; nt < NT; ++nt) {
-                                    const uint2 q = qf[(nt * C::STEPS + st) * 32 + lane];
-                                    mma_bf16_16816(sc[e][nt], a0, a1, a2, a3, q.x, q.y);
-                                }
-                            }
-                        } else {
-                            const int st = p * NWK + w;
-                            const uint32_t a0 = dequant8(w0v[w], s0, b0), a2 = dequant8(w0v[w] >> 8, s0, b0);
-                            const uint32_t a1 = dequant8(w1v[w], s1, b1), a3 = dequant8(w1v[w] >> 8, s1, b1);
-#pragma unroll
-                            for (int nt = 0; nt < NT; ++nt) {
-                                const uint2 q = qf[(nt * C::STEPS + st) * 32 + lane];
-                                mma_bf16_16816(sc[e][nt], a0, a1, a2, a3, q.x, q.y);
-                            }
+                        for (int w = 0; w < 2; ++w) {
+                            f0[4 * w] = lop3_and_or(xs[w], 0x000F000Fu, kF16Magic);
+                            f0[4 * w + 1] = lop3_and_or(xs[w], 0x00F000F0u, kF16Magic);
+                            f0[4 * w + 2] = lop3_and_or(xs[w] >> 8, 0x000F000Fu, kF16Magic);
+                            f0[4 * w + 3] = lop3_and_or(xs[w] >> 8, 0x00F000F0u, kF16Magic);
+                            f1[4 * w] = lop3_and_or(ys[w], 0x000F000Fu, kF16Magic);
+                            f1[4 * w + 1] = lop3_and_or(ys[w], 0x00F000F0u, kF16Magic);
+                            f1[4 * w + 2] = lop3_and_or(ys[w] >> 8, 0x000F000Fu, kF16Magic);
+                            f1[4 * w + 3] = lop3_and_or(ys[w] >> 8, 0x00F000F0u, kF16Magic);
                         }
+                    } else {
+                        const uint4 x = lds128(u + gr * 1024 + g * 64 + t * 16), y = lds128(u + gr * 1024 + (g + 8) * 64 + t * 16);
+                        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                        for (int w = 0; w < 4; ++w) {
+                            f0[2 * w] = __byte_perm(xs[w], kF16MagicBytes, 0x4140);
+                            f0[2 * w + 1] = __byte_perm(xs[w], kF16MagicBytes, 0x4342);
+                            f1[2 * w] = __byte_perm(ys[w], kF16MagicBytes, 0x4140);
+                            f1[2 * w + 1] = __byte_perm(ys[w], kF16MagicBytes, 0x4342);
+                        }
+                    }
+                    const float s0 = pair_scale(p0[gr]), b0 = pair_bias(p0[gr]), s1 = pair_scale(p1[gr]), b1 = pair_bias(p1[gr]);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        const float4 qs = *reinterpret_cast<const float4*>(&qsum[((nt * G + gr) * 4 + t) * 2]);
+                        float acc[4] = {qs.y, qs.w, qs.y, qs.w};
+#pragma unroll
+                        for (int st = 0; st < 4; ++st) {
+                            const uint2 q = qf[((nt * G + gr) * 4 + st) * 32 + lane];
+                            mma_f16_16816(acc, f0[2 * st], f1[2 * st], f0[2 * st + 1], f1[2 * st + 1], q.x, q.y);
+                        }
+                        sc[e][nt][0] = fmaf(s0, acc[0], fmaf(b0, qs.x, sc[e][nt][0]));
+                        sc[e][nt][1] = fmaf(s0, acc[1], fmaf(b0, qs.z, sc[e][nt][1]));
+                        sc[e][nt][2] = fmaf(s1, acc[2], fmaf(b1, qs.x, sc[e][nt][2]));
+                        sc[e][nt][3] = fmaf(s1, acc[3], fmaf(b1, qs.z, sc[e][nt][3]));
                     }
                 }
             }
             if (!ok) break;
-            // scores in units of log2, masked where a row does not see the position
-            const int pos = unit_of(k) * kKvRows;
-            const bool mask = pos + 2 * kKvRows > min(first_seen, s.len) || !two;
+            // scores in units of log2, masked where a row does not see the position; the exponent of the
+            // largest scale of the values (rows behind the last position may hold anything and are left out)
+            const bool mask = pos + 2 * kKvRows > first_seen || !two;
+            uint32_t big = 0;
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
+            for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    uint32_t w = *reinterpret_cast<const uint32_t*>(up[e] + kv_value_pair(g + 8 * x, t % G, C::RB, G)) & 0x7fffu;
+                    if (mask && (pos + e * kKvRows + g + 8 * x >= s.len || (e == 1 && !two))) w = 0;
+                    big = max(big, w);
+                }
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int x = 0; x < 4; ++x) {
-                        sc[e][nt][x] *= a.scale_log2;
+                        sc[e][nt][x] *= sr[nt][x & 1];
                         if (mask && (pos + e * kKvRows + g + (x >> 1) * 8 >= lim[nt][x & 1] || (e == 1 && !two))) sc[e][nt][x] = -INFINITY;
                     }
+            }
+            big = __reduce_max_sync(0xffffffffu, big);
+            const float ex = (float)max((int)(big >> 7) - 127, -60);
             bool grew = false;
-            float mu[NT][2], up_by[NT][2];
+            float mu[NT][2], by[NT][2];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -303,99 +389,107 @@ __global__ void __launch_bounds__(kThreads, StepCfg<D, BITS, NT>::CTAS) attn_ste
                     float mx = fmaxf(fmaxf(sc[0][nt][x], sc[0][nt][x + 2]), fmaxf(sc[1][nt][x], sc[1][nt][x + 2]));
 #pragma unroll
                     for (int of = 4; of < 32; of <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, of));
-                    const float mn = fmaxf(m[nt][x], mx);
+                    const float mn = fmaxf(m[nt][x], mx + ex);
                     grew |= mn > m[nt][x];
                     mu[nt][x] = mn == -INFINITY ? 0.f : mn;
-                    up_by[nt][x] = ex2(m[nt][x] - mu[nt][x]);
+                    by[nt][x] = ex2(m[nt][x] - mu[nt][x]);
                     m[nt][x] = mn;
                 }
             if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
-                    for (int x = 0; x < 2; ++x) l[nt][x] *= up_by[nt][x];
+                    for (int x = 0; x < 2; ++x) {
+                        l[nt][x] *= by[nt][x];
+#pragma unroll
+                        for (int gr = 0; gr < G; ++gr) bs[nt][gr][x] *= by[nt][x];
+                    }
 #pragma unroll
                     for (int j = 0; j < D / 16; ++j)
 #pragma unroll
-                        for (int x = 0; x < 4; ++x) o[nt][j][x] *= up_by[nt][x & 1];
+                        for (int x = 0; x < 4; ++x) o[nt][j][x] *= by[nt][x & 1];
                 }
             }
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 if (e == 1 && !two) continue;
-                uint32_t pb[NT][2];
+                float p[NT][4];
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    float p[4];
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int x = 0; x < 4; ++x) {
-                        p[x] = ex2(sc[e][nt][x] - mu[nt][x & 1]);
-                        l[nt][x & 1] += p[x];
+                        p[nt][x] = ex2(sc[e][nt][x] - mu[nt][x & 1]);
+                        l[nt][x & 1] += p[nt][x];
                     }
-                    pb[nt][0] = movmatrix(bf16x2_of(p[0], p[1]));
-                    pb[nt][1] = movmatrix(bf16x2_of(p[2], p[3]));
-                }
                 const uint8_t* u = up[e];
-                constexpr int NW = C::RB / 32;  // words per lane and row
-                uint32_t vw[4][NW], pr[4];
-                const int key0 = pos + e * kKvRows;
+                uint32_t p0[G], p1[G];
+                load_pairs<G>(u + kv_value_pair(g, 0, C::RB, G), p0);
+                load_pairs<G>(u + kv_value_pair(g + 8, 0, C::RB, G), p1);
+                if (mask) {  // a row behind the last position, as zeros, adds nothing
+                    const int key = pos + e * kKvRows + g;
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int r = 2 * t + (q & 1) + (q >> 1) * 8;
-                    pr[q] = *reinterpret_cast<const uint32_t*>(u + kv_value_pair(r, g * (D / 8) / 64, C::RB, C::G));
-                    // a row behind the last position may hold anything; as zeros it adds nothing
-                    if (key0 + r >= s.len) pr[q] = 0u;
-                    const uint8_t* vb = u + kKvRows * (C::RB + 4 * C::G) + (q * 8 + t) * 16;
-                    if constexpr (NW == 1) {
-                        vw[q][0] = *reinterpret_cast<const uint32_t*>(vb + (g >> 2) * 64 + (g & 3) * 4);
-                    } else if constexpr (NW == 2) {
-                        const uint2 x = lds64(vb + (g >> 2) * 512 + ((g >> 1) & 1) * 64 + (g & 1) * 8);
-                        vw[q][0] = x.x, vw[q][1] = x.y;
-                    } else if constexpr (NW == 4) {
-                        const uint4 x = lds128(vb + (g >> 1) * 512 + (g & 1) * 64);
-                        vw[q][0] = x.x, vw[q][1] = x.y, vw[q][2] = x.z, vw[q][3] = x.w;
-                    } else {  // two pieces, odd lanes take them in the other order (no bank conflict)
-#pragma unroll
-                        for (int c = 0; c < 2; ++c) {
-                            const uint4 x = lds128(vb + g * 512 + (c ^ (g & 1)) * 64);
-                            vw[q][4 * c] = x.x, vw[q][4 * c + 1] = x.y, vw[q][4 * c + 2] = x.z, vw[q][4 * c + 3] = x.w;
-                        }
+                    for (int gr = 0; gr < G; ++gr) {
+                        if (key >= s.len) p0[gr] = 0u;
+                        if (key + 8 >= s.len) p1[gr] = 0u;
                     }
                 }
-                const uint32_t s01 = __byte_perm(pr[0], pr[1], 0x5410), b01 = __byte_perm(pr[0], pr[1], 0x7632);
-                const uint32_t s23 = __byte_perm(pr[2], pr[3], 0x5410), b23 = __byte_perm(pr[2], pr[3], 0x7632);
+                const uint8_t* vb = u + kKvRows * (C::RB + 4 * G) + t * 16;
 #pragma unroll
-                for (int w = 0; w < NW; ++w) {
+                for (int gr = 0; gr < G; ++gr) {
+                    // eight features of the rows 2t, 2t + 1 (low and high half) and 2t + 8, 2t + 9
+                    uint32_t f01[8], f23[8];
                     if (BITS == 4) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int q = 0; q < 4; ++q)
+                            w[q] = *reinterpret_cast<const uint32_t*>(vb + gr * 512 + q * 128 + (g >> 2) * 64 + (g & 3) * 4);
 #pragma unroll
                         for (int hf = 0; hf < 2; ++hf) {
-                            const uint32_t x01 = __byte_perm(vw[0][w], vw[1][w], hf ? 0x7632 : 0x5410);
-                            const uint32_t x23 = __byte_perm(vw[2][w], vw[3][w], hf ? 0x7632 : 0x5410);
+                            const uint32_t x01 = __byte_perm(w[0], w[1], hf ? 0x7632 : 0x5410), x23 = __byte_perm(w[2], w[3], hf ? 0x7632 : 0x5410);
 #pragma unroll
                             for (int y = 0; y < 2; ++y) {
-                                const uint32_t a0 = dequant4(x01 >> (8 * y), s01, b01), a1 = dequant4(x01 >> (8 * y + 4), s01, b01);
-                                const uint32_t a2 = dequant4(x23 >> (8 * y), s23, b23), a3 = dequant4(x23 >> (8 * y + 4), s23, b23);
-#pragma unroll
-                                for (int nt = 0; nt < NT; ++nt)
-                                    mma_bf16_16816(o[nt][w * 4 + hf * 2 + y], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
+                                const uint32_t a01 = y ? x01 >> 8 : x01, a23 = y ? x23 >> 8 : x23;
+                                f01[hf * 4 + y * 2] = f16x2_add(lop3_and_or(a01, 0x000F000Fu, kF16Magic), kF16Neg1032x2);
+                                f01[hf * 4 + y * 2 + 1] = f16x2_add(lop3_and_or(a01, 0x00F000F0u, kF16Magic), kF16Neg1152x2);
+                                f23[hf * 4 + y * 2] = f16x2_add(lop3_and_or(a23, 0x000F000Fu, kF16Magic), kF16Neg1032x2);
+                                f23[hf * 4 + y * 2 + 1] = f16x2_add(lop3_and_or(a23, 0x00F000F0u, kF16Magic), kF16Neg1152x2);
                             }
                         }
                     } else {
+                        uint2 w[4];
 #pragma unroll
-                        for (int y = 0; y < 2; ++y) {
-                            const uint32_t s0 = 2 * y, s1 = 2 * y + 1;  // byte n of both rows to bits [0,8) and [16,24)
-                            const uint32_t a0 = dequant8(__byte_perm(vw[0][w], vw[1][w], s0 | (4 + s0) << 8), s01, b01);
-                            const uint32_t a1 = dequant8(__byte_perm(vw[0][w], vw[1][w], s1 | (4 + s1) << 8), s01, b01);
-                            const uint32_t a2 = dequant8(__byte_perm(vw[2][w], vw[3][w], s0 | (4 + s0) << 8), s23, b23);
-                            const uint32_t a3 = dequant8(__byte_perm(vw[2][w], vw[3][w], s1 | (4 + s1) << 8), s23, b23);
+                        for (int q = 0; q < 4; ++q)
+                            w[q] = lds64(vb + (2 * gr + (g >> 2)) * 512 + q * 128 + ((g >> 1) & 1) * 64 + (g & 1) * 8);
 #pragma unroll
-                            for (int nt = 0; nt < NT; ++nt)
-                                mma_bf16_16816(o[nt][w * 2 + y], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
+                        for (int hf = 0; hf < 2; ++hf) {
+                            const uint32_t w0 = hf ? w[0].y : w[0].x, w1 = hf ? w[1].y : w[1].x;
+                            const uint32_t w2 = hf ? w[2].y : w[2].x, w3 = hf ? w[3].y : w[3].x;
+#pragma unroll
+                            for (int y = 0; y < 2; ++y) {
+                                const uint32_t a01 = __byte_perm(w0, w1, y ? 0x7362 : 0x5140), a23 = __byte_perm(w2, w3, y ? 0x7362 : 0x5140);
+                                f01[hf * 4 + y * 2] = f16x2_add(__byte_perm(a01, kF16MagicBytes, 0x4140), kF16Neg1152x2);
+                                f01[hf * 4 + y * 2 + 1] = f16x2_add(__byte_perm(a01, kF16MagicBytes, 0x4342), kF16Neg1152x2);
+                                f23[hf * 4 + y * 2] = f16x2_add(__byte_perm(a23, kF16MagicBytes, 0x4140), kF16Neg1152x2);
+                                f23[hf * 4 + y * 2 + 1] = f16x2_add(__byte_perm(a23, kF16MagicBytes, 0x4342), kF16Neg1152x2);
+                            }
                         }
+                    }
+                    constexpr float kMid = BITS == 4 ? 8.f : 128.f;
+                    const float s0 = pair_scale(p0[gr]), s1 = pair_scale(p1[gr]);
+                    const float b0 = fmaf(kMid, s0, pair_bias(p0[gr])), b1 = fmaf(kMid, s1, pair_bias(p1[gr]));
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        bs[nt][gr][0] = fmaf(p[nt][0], b0, fmaf(p[nt][2], b1, bs[nt][gr][0]));
+                        bs[nt][gr][1] = fmaf(p[nt][1], b0, fmaf(p[nt][3], b1, bs[nt][gr][1]));
+                        const uint32_t q0 = movmatrix(f16x2_of(p[nt][0] * s0, p[nt][1] * s0));
+                        const uint32_t q1 = movmatrix(f16x2_of(p[nt][2] * s1, p[nt][3] * s1));
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            mma_f16_16816(o[nt][gr * 4 + j], f01[2 * j], f01[2 * j + 1], f23[2 * j], f23[2 * j + 1], q0, q1);
                     }
                 }
             }
-            __syncwarp();  // both slots are read by every lane before lane 0 refills them
+            __syncwarp();  // both slots are read by every lane before they are refilled
             issue(min(mine, k + 2 + C::RING));
         }
         if (!ok) {  // a copy did not arrive (recorded): give the others in flight their time, then leave
@@ -410,9 +504,14 @@ __global__ void __launch_bounds__(kThreads, StepCfg<D, BITS, NT>::CTAS) attn_ste
 #pragma unroll
             for (int x = 0; x < 2; ++x)
 #pragma unroll
-                for (int of = 4; of < 32; of <<= 1) l[nt][x] += __shfl_xor_sync(0xffffffffu, l[nt][x], of);
+                for (int of = 4; of < 32; of <<= 1) {
+                    l[nt][x] += __shfl_xor_sync(0xffffffffu, l[nt][x], of);
+#pragma unroll
+                    for (int gr = 0; gr < G; ++gr) bs[nt][gr][x] += __shfl_xor_sync(0xffffffffu, bs[nt][gr][x], of);
+                }
         __syncthreads();
         if (stop) return;
+        constexpr float kOdd = BITS == 4 ? 0.0625f : 1.0f;  // odd features were summed 16-fold
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -421,16 +520,16 @@ __global__ void __launch_bounds__(kThreads, StepCfg<D, BITS, NT>::CTAS) attn_ste
                 if (g == 0) ml[warp * C::ROWS + r] = make_float2(m[nt][x], l[nt][x]);
 #pragma unroll
                 for (int i = 0; i < D / 32; ++i) {
-                    // float4 i of lane g's features, placed at i 8 + (g + r & ~1) % 8: conflict-free both ways
-                    int at = i;
-                    if (D == 256 && BITS == 8 && (g & 1)) at = i ^ 4;  // odd lanes hold their two pieces swapped
-                    merge[(warp * C::ROWS + r) * (D / 4) + at * 8 + ((g + (r & ~1)) & 7)] =
-                        make_float4(o[nt][2 * i][x], o[nt][2 * i][x + 2], o[nt][2 * i + 1][x], o[nt][2 * i + 1][x + 2]);
+                    // features 64 (i / 2) + 8 g + 4 (i % 2) .. + 3, placed at i 8 + (g + r & ~1) % 8: no conflict
+                    const float z = bs[nt][i / 2][x];
+                    merge[(warp * C::ROWS + r) * (D / 4) + i * 8 + ((g + (r & ~1)) & 7)] =
+                        make_float4(o[nt][2 * i][x] + z, fmaf(o[nt][2 * i][x + 2], kOdd, z), o[nt][2 * i + 1][x] + z,
+                                    fmaf(o[nt][2 * i + 1][x + 2], kOdd, z));
                 }
             }
         __syncthreads();
         for (int i = tid; i < nrows * (D / 4); i += kThreads) {
-            const int r = i / (D / 4), f = i % (D / 4), gg = f / (D / 32), at = f % (D / 32);
+            const int r = i / (D / 4), f = i % (D / 4), gg = (f >> 1) & 7, at = (f >> 4) * 2 + (f & 1);
             float mx = -INFINITY;
 #pragma unroll
             for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, ml[w * C::ROWS + r].x);
@@ -447,8 +546,7 @@ __global__ void __launch_bounds__(kThreads, StepCfg<D, BITS, NT>::CTAS) attn_ste
             }
             if (whole) {
                 const float inv = sum == 0.f ? 0.f : 1.f / sum;
-                const int rr = row0 + r;
-                uint16_t* y = a.out + ((int64_t)(s.q0 + rr / a.group) * a.heads + h * a.group + rr % a.group) * D + f * 4;
+                uint16_t* y = a.out + ((int64_t)(s.q0 + r / a.group) * a.heads + h * a.group + r % a.group) * D + f * 4;
                 *reinterpret_cast<uint2*>(y) = make_uint2(bf16x2_of(acc.x * inv, acc.y * inv), bf16x2_of(acc.z * inv, acc.w * inv));
             } else {
                 reinterpret_cast<float4*>(work.o)[((int64_t)slot * C::ROWS + r) * (D / 4) + f] = acc;
@@ -460,81 +558,74 @@ __global__ void __launch_bounds__(kThreads, StepCfg<D, BITS, NT>::CTAS) attn_ste
     }
 }
 
-// Joins a tile's partial rows.  Block (i, r): row r of the tile that share boundary i cuts, if i is the
-// first boundary inside it.
+// Joins the partial rows of tile (sequence, kv head) blockIdx.x, if it was cut.  gridDim.y blocks share its
+// (row, 64 features) parts; in a block 16 lanes take 4 features each, 16 lane groups every 16th partial.
 template <int D>
 __global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ AttnArgs a, int grid, int rows) {
-    constexpr int F = D / 4, GROUPS = 256 / F;
-    __shared__ uint32_t pre[kAttnMaxBatch + 1];
-    __shared__ float wgt[2048];
+    constexpr int F = 16, GROUPS = 256 / F;
+    __shared__ float wgt[1024];
     __shared__ float4 acc_s[256];
-    __shared__ float red[256];
+    __shared__ float2 red[8];
     const int tid = threadIdx.x;
     pdl_wait();
     pdl_launch_dependents();
     const StepWork work = step_work(a.part, grid, rows);
-    for (int b = tid; b <= a.batch; b += 256) pre[b] = work.prefix[b];
-    const uint32_t share = work.prefix[kAttnMaxBatch + 1];
-    __syncthreads();
-    const uint64_t w = (uint64_t)(blockIdx.x + 1) * share;
-    if (w >= pre[a.batch]) return;
-    int lo = 0, hi = a.batch - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (pre[mid] <= w) lo = mid; else hi = mid - 1;
-    }
-    const int b = lo;
+    const int b = blockIdx.x / a.pool.kv_heads, h = blockIdx.x % a.pool.kv_heads;
+    const uint32_t from = work.prefix[b], share = work.prefix[kAttnMaxBatch + 1];
+    const uint32_t vl = (work.prefix[b + 1] - from) / a.pool.kv_heads;
+    if (vl == 0) return;
+    const uint32_t first = from + h * vl, c0 = (first + kTileCost) / share, c1 = (first + vl - 1) / share;
+    if (c0 == c1) return;  // one CTA did all of it
     const SeqSpan s = seq_span(a, b);
-    const uint32_t nu = (uint32_t)((s.len + kKvRows - 1) / kKvRows);
-    const uint32_t tiles = (uint32_t)((s.n * a.group + rows - 1) / rows);
-    const uint32_t ti = ((uint32_t)w - pre[b]) / nu, first = pre[b] + ti * nu;
-    if (first == w || (uint64_t)blockIdx.x * share > first) return;  // no cut here, or an earlier one joins it
-    const int h = (int)(ti / tiles), row = (int)(ti % tiles) * rows + (int)blockIdx.y;
-    if (row >= s.n * a.group) return;
-    const uint32_t c0 = first / share, n = (first + nu - 1) / share - c0 + 1;
+    const uint32_t n = c1 - c0 + 1;
     auto slot_of = [&](uint32_t i) { return 2 * (c0 + i) + ((uint64_t)(c0 + i) * share >= first ? 0 : 1); };
-    float mx = -INFINITY;
-    for (uint32_t i = tid; i < n; i += 256) mx = fmaxf(mx, work.ml[slot_of(i) * rows + blockIdx.y].x);
-    red[tid] = mx;
-    __syncthreads();
-    for (int o = 128; o; o >>= 1) {
-        if (tid < o) red[tid] = fmaxf(red[tid], red[tid + o]);
-        __syncthreads();
-    }
-    mx = red[0] == -INFINITY ? 0.f : red[0];
-    __syncthreads();
-    float sum = 0.f;
-    for (uint32_t i = tid; i < n; i += 256) {
-        const float2 e = work.ml[slot_of(i) * rows + blockIdx.y];
-        const float f = ex2(e.x - mx);
-        wgt[i] = f;
-        sum += f * e.y;
-    }
-    red[tid] = sum;
-    __syncthreads();
-    for (int o = 128; o; o >>= 1) {
-        if (tid < o) red[tid] += red[tid + o];
-        __syncthreads();
-    }
-    sum = red[0];
     const int f = tid % F, grp = tid / F;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (uint32_t i = grp; i < n; i += GROUPS) {
-        const float4 v = reinterpret_cast<const float4*>(work.o)[((int64_t)slot_of(i) * rows + blockIdx.y) * F + f];
-        const float g = wgt[i];
-        acc.x += g * v.x, acc.y += g * v.y, acc.z += g * v.z, acc.w += g * v.w;
+    for (int part = blockIdx.y; part < s.n * a.group * (D / 64); part += gridDim.y) {
+        const int row = part / (D / 64), fo = part % (D / 64) * 16 + f;
+        float mx = -INFINITY;
+        for (uint32_t i = tid; i < n; i += 256) mx = fmaxf(mx, work.ml[slot_of(i) * rows + row].x);
+#pragma unroll
+        for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        if (tid % 32 == 0) red[tid / 32].x = mx;
+        __syncthreads();
+        mx = red[0].x;
+#pragma unroll
+        for (int i = 1; i < 8; ++i) mx = fmaxf(mx, red[i].x);
+        if (mx == -INFINITY) mx = 0.f;
+        float sum = 0.f;
+        for (uint32_t i = tid; i < n; i += 256) {
+            const float2 e = work.ml[slot_of(i) * rows + row];
+            const float w = ex2(e.x - mx);
+            wgt[i] = w;
+            sum += w * e.y;
+        }
+#pragma unroll
+        for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (tid % 32 == 0) red[tid / 32].y = sum;
+        __syncthreads();
+        sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum += red[i].y;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+        for (uint32_t i = grp; i < n; i += GROUPS) {
+            const float4 v = reinterpret_cast<const float4*>(work.o)[((int64_t)slot_of(i) * rows + row) * (D / 4) + fo];
+            const float w = wgt[i];
+            acc.x += w * v.x, acc.y += w * v.y, acc.z += w * v.z, acc.w += w * v.w;
+        }
+        acc_s[tid] = acc;
+        __syncthreads();
+        if (grp == 0) {
+            for (int i = 1; i < GROUPS; ++i) {
+                const float4 v = acc_s[i * F + f];
+                acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
+            }
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            uint16_t* y = a.out + ((int64_t)(s.q0 + row / a.group) * a.heads + h * a.group + row % a.group) * D + fo * 4;
+            *reinterpret_cast<uint2*>(y) = make_uint2(bf16x2_of(acc.x * inv, acc.y * inv), bf16x2_of(acc.z * inv, acc.w * inv));
+        }
+        __syncthreads();
     }
-    acc_s[tid] = acc;
-    __syncthreads();
-    if (grp) return;
-    for (int i = 1; i < GROUPS; ++i) {
-        const float4 v = acc_s[i * F + f];
-        acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
-    }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    uint16_t* y = a.out + ((int64_t)(s.q0 + row / a.group) * a.heads + h * a.group + row % a.group) * D + f * 4;
-    *reinterpret_cast<uint2*>(y) = make_uint2(bf16x2_of(acc.x * inv, acc.y * inv), bf16x2_of(acc.z * inv, acc.w * inv));
 }
 
 template <typename... P, typename... A>
@@ -560,37 +651,35 @@ cudaError_t run_step(const AttnArgs& a, cudaStream_t stream) {
     cudaError_t e = cudaFuncSetAttribute(attn_step_kernel<D, BITS, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM);
     if (e != cudaSuccess) return e;
     // no more CTAs than the longest lengths the table can hold would occupy
-    const int64_t tiles = (int64_t)a.pool.kv_heads * (a.tokens * a.group / C::ROWS + a.batch);
-    const int64_t most = tiles * a.table_width * a.pool.page_units;
-    const int grid = (int)std::max<int64_t>(1, std::min<int64_t>((int64_t)device_num_sms() * C::CTAS, (most + kMinShare - 1) / kMinShare));
+    const int tiles = a.batch * a.pool.kv_heads, sms = device_num_sms();
+    const int64_t most = tiles * ((int64_t)a.table_width * a.pool.page_units + kTileCost);
+    const int grid = (int)std::max<int64_t>(1, std::min<int64_t>((int64_t)sms * C::CTAS, (most + kMinShare - 1) / kMinShare));
     e = launch_attn(attn_step_kernel<D, BITS, NT>, dim3(grid), kThreads, C::SMEM, a.pdl, stream, a);
     if (e != cudaSuccess || grid == 1) return e;
-    return launch_attn(attn_join_kernel<D>, dim3(grid - 1, C::ROWS), 256, 0, a.pdl, stream, a, grid, (int)C::ROWS);
+    const int parts = std::max(1, std::min(4 * sms / tiles, a.max_q * a.group * (D / 64)));
+    return launch_attn(attn_join_kernel<D>, dim3(tiles, parts), 256, 0, a.pdl, stream, a, grid, (int)C::ROWS);
 }
 
 template <int D, int BITS>
 cudaError_t run_rows(const AttnArgs& a, cudaStream_t stream) {
-    return (int64_t)a.max_q * a.group <= 8 ? run_step<D, BITS, 1>(a, stream) : run_step<D, BITS, 2>(a, stream);
+    return a.max_q * a.group <= 8 ? run_step<D, BITS, 1>(a, stream) : run_step<D, BITS, 2>(a, stream);
 }
 
 }  // namespace
 
-size_t attn_workspace_bytes(int64_t tokens, int heads, int kv_heads, int dim, int batch) {
+bool step_applies(const AttnArgs& a) { return (int64_t)a.max_q * a.group <= 16; }
+
+size_t step_workspace_bytes(int dim) {
     return kStepHead + (size_t)2 * device_num_sms() * kStepMaxCtas * 16 * (dim * 4 + 8);
 }
 
-bool attention_applies(const AttnArgs& a) {
-    const int64_t tiles = (int64_t)a.pool.kv_heads * (a.tokens * a.group / 8 + a.batch);
-    return (double)tiles * a.table_width * a.pool.page_units < 4.0e9;
-}
-
-cudaError_t launch_paged_attention(const AttnArgs& a, cudaStream_t stream) {
+cudaError_t launch_attn_step(const AttnArgs& a, cudaStream_t stream) {
     const bool b4 = a.pool.bits == 4;
     if (a.pool.dim == 64) return b4 ? run_rows<64, 4>(a, stream) : run_rows<64, 8>(a, stream);
     if (a.pool.dim == 128) return b4 ? run_rows<128, 4>(a, stream) : run_rows<128, 8>(a, stream);
     return b4 ? run_rows<256, 4>(a, stream) : run_rows<256, 8>(a, stream);
 }
 
-int attn_device_error(bool clear) { return tu_device_error(clear); }
+int step_device_error(bool clear) { return tu_device_error(clear); }
 
 }  // namespace marlin

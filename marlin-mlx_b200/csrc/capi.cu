@@ -169,14 +169,15 @@ int marlin_q4_device_error(int clear) {
     const int v_i8 = i8_device_error(clear != 0), v_pf = prefill_device_error(clear != 0),
               v_mi = misc_device_error(clear != 0), v_fu = fused_device_error(clear != 0),
               v_ro = rows_device_error(clear != 0), v_kv = kv_device_error(clear != 0),
-              v_at = attn_device_error(clear != 0);
+              v_st = step_device_error(clear != 0), v_ch = chunk_device_error(clear != 0);
     if (!v) v = v_fu;
     if (!v) v = v_ro;
     if (!v) v = v_i8;
     if (!v) v = v_pf;
     if (!v) v = v_mi;
     if (!v) v = v_kv;
-    if (!v) v = v_at;
+    if (!v) v = v_st;
+    if (!v) v = v_ch;
     if (v < 0) return cuda_status(cudaGetLastError());
     return v;
 }
@@ -328,7 +329,7 @@ size_t marlin_q4_paged_attention_workspace_size(int64_t tokens, int32_t heads, i
     if (tokens < 0 || tokens > kMaxTokens || heads <= 0 || heads > kMaxHeads || kv_heads <= 0 || heads % kv_heads != 0 ||
         !kv_dims(head_dim, 4) || batch <= 0 || batch > kAttnMaxBatch)
         return 0;
-    return align16(attn_workspace_bytes(tokens, heads, kv_heads, head_dim, batch));
+    return align16(std::max(step_workspace_bytes(head_dim), chunk_workspace_bytes(tokens, heads, kv_heads, head_dim, batch)));
 }
 
 int marlin_q4_paged_attention(const uint16_t* q, int64_t q_token_stride, int64_t q_head_stride,
@@ -372,8 +373,9 @@ int marlin_q4_paged_attention(const uint16_t* q, int64_t q_token_stride, int64_t
     a.out = out;
     a.part = static_cast<float*>(workspace);
     a.pdl = g_pdl;
-    if (!attention_applies(a)) return MARLIN_Q4_ERR_UNSUPPORTED;
-    return cuda_status(launch_paged_attention(a, static_cast<cudaStream_t>(stream)));
+    if (step_applies(a)) return cuda_status(launch_attn_step(a, static_cast<cudaStream_t>(stream)));
+    if (!chunk_fits(a)) return MARLIN_Q4_ERR_UNSUPPORTED;
+    return cuda_status(launch_attn_chunk(a, static_cast<cudaStream_t>(stream)));
 }
 
 int marlin_q4_rms_norm(const void* x, int32_t x_dtype, const uint16_t* weight, int64_t m, int64_t h, float eps,

@@ -91,11 +91,17 @@ struct AttnArgs {
     bool pdl;
 };
 constexpr int kAttnMaxBatch = 1024;
-size_t attn_workspace_bytes(int64_t tokens, int heads, int kv_heads, int dim, int batch);
-bool attention_applies(const AttnArgs& a);  // the work's index fits its 32 bits
-cudaError_t launch_paged_attention(const AttnArgs& a, cudaStream_t stream);
+// Few rows: at most 16 (token, head of the group) rows per sequence and kv head.
+bool step_applies(const AttnArgs& a);
+size_t step_workspace_bytes(int dim);
+cudaError_t launch_attn_step(const AttnArgs& a, cudaStream_t stream);
+// Any number of rows.
+bool chunk_fits(const AttnArgs& a);  // the tiles' index fits its 32 bits
+size_t chunk_workspace_bytes(int64_t tokens, int heads, int kv_heads, int dim, int batch);
+cudaError_t launch_attn_chunk(const AttnArgs& a, cudaStream_t stream);
 
 int kv_device_error(bool clear);
-int attn_device_error(bool clear);
+int step_device_error(bool clear);
+int chunk_device_error(bool clear);
 
 }  // namespace marlin

@@ -56,12 +56,15 @@ def norm_rope(x, w, positions, freqs, eps, interleaved, axes=None):
 
 
 def attention(q, ks, vs, lens, starts, scale):
-    """q [tokens, heads, dim]; ks, vs: per sequence [len, kv_heads, dim].  Returns (out, mix, spread): the
-    attention, sum p |v| and the largest scale * sum |q| |k| over the row's positions (what errors scale with)."""
-    out, mix, spread = np.zeros_like(q), np.zeros_like(q), np.zeros(q.shape[:2])
+    """q [tokens, heads, dim]; ks, vs: per sequence [len, kv_heads, dim].  Returns (out, mix, top, spread): the
+    attention; sum p |v|; the same with each |v| raised to the largest of its 64-feature group; and the
+    largest scale * sum |q| |k| over the row's positions (what errors scale with)."""
+    out, mix, top = np.zeros_like(q), np.zeros_like(q), np.zeros_like(q)
+    spread = np.zeros(q.shape[:2])
     for b, n_pos in enumerate(lens):
         n = starts[b + 1] - starts[b]
         group = q.shape[1] // ks[b].shape[1]
+        raised = np.abs(vs[b]).reshape(n_pos, ks[b].shape[1], q.shape[2] // GROUP, GROUP).max(-1).repeat(GROUP, -1)
         for i in range(n):
             seen = n_pos - n + i + 1
             if seen <= 0:
@@ -72,6 +75,6 @@ def attention(q, ks, vs, lens, starts, scale):
                 x = scale * (k @ q[t, h])
                 p = np.exp(x - x.max())
                 p /= p.sum()
-                out[t, h], mix[t, h] = p @ v, p @ np.abs(v)
+                out[t, h], mix[t, h], top[t, h] = p @ v, p @ np.abs(v), p @ raised[:seen, h // group]
                 spread[t, h] = scale * (np.abs(k) @ np.abs(q[t, h])).max()
-    return out, mix, spread
+    return out, mix, top, spread
