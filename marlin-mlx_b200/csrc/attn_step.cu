@@ -107,7 +107,7 @@ __device__ __forceinline__ float pair_scale(uint32_t w) { return __uint_as_float
 __device__ __forceinline__ float pair_bias(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
 
 template <int D, int BITS, int NT>
-__global__ void __launch_bounds__(kThreads, StepCfg<D, BITS, NT>::CTAS) attn_step_kernel(const __grid_constant__ AttnArgs a) {
+__global__ void __launch_bounds__(kThreads, StepCfg<D, BITS, NT>::CTAS) attn_step_kernel(const __grid_constant__ AttnArgs a, int whole_tiles) {
     using C = StepCfg<D, BITS, NT>;
     constexpr int G = C::G;
     extern __shared__ __align__(128) uint8_t smem[];
@@ -130,10 +130,18 @@ __global__ void __launch_bounds__(kThreads, StepCfg<D, BITS, NT>::CTAS) attn_ste
     }
     pdl_wait();
     pdl_launch_dependents();
-    // prefix sums of the sequences' work
+    // prefix sums of the sequences' work (whole_tiles: CTA i does tile i, and its sequence is all there is)
     uint32_t base = 0;
     if (tid == 0) pre[0] = 0;
-    for (int b0 = 0; b0 < a.batch; b0 += kThreads) {
+    const int only = (int)blockIdx.x / a.pool.kv_heads;
+    if (whole_tiles) {
+        const SeqSpan s = seq_span(a, only);
+        if (s.len == 0 && (int)blockIdx.x % a.pool.kv_heads == 0)
+            for (int64_t i = tid; i < (int64_t)s.n * a.heads * D / 8; i += kThreads)
+                reinterpret_cast<uint4*>(a.out + (int64_t)s.q0 * a.heads * D)[i] = make_uint4(0u, 0u, 0u, 0u);
+        base = tile_work(s) * (uint32_t)a.pool.kv_heads;
+    }
+    for (int b0 = 0; b0 < a.batch && !whole_tiles; b0 += kThreads) {
         const int b = b0 + tid;
         uint32_t v = 0;
         if (b < a.batch) {
@@ -163,27 +171,27 @@ __global__ void __launch_bounds__(kThreads, StepCfg<D, BITS, NT>::CTAS) attn_ste
     }
     __syncthreads();
     const uint32_t total = base;
-    const uint32_t share = max(kMinShare, (total + gridDim.x - 1) / gridDim.x);
+    const uint32_t share = whole_tiles ? total / a.pool.kv_heads : max(kMinShare, (total + gridDim.x - 1) / gridDim.x);
     const StepWork work = step_work(a.part, gridDim.x, C::ROWS);
-    if (blockIdx.x == 0) {
+    if (blockIdx.x == 0 && !whole_tiles) {
         for (int b = tid; b <= a.batch; b += kThreads) work.prefix[b] = pre[b];
         if (tid == 0) work.prefix[kAttnMaxBatch + 1] = share;
     }
-    const uint64_t w_begin = (uint64_t)blockIdx.x * share;
+    const uint64_t w_begin = (uint64_t)(whole_tiles ? (int)blockIdx.x % a.pool.kv_heads : (int)blockIdx.x) * share;
     const uint32_t w_end = (uint32_t)min((uint64_t)total, w_begin + share);
 
     uint32_t done = 0;  // units this warp has consumed so far (ring position and phase)
     for (uint32_t w0 = (uint32_t)min(w_begin, (uint64_t)total); w0 < w_end;) {
         // the range's sequence, kv head and units; a tile's first kTileCost steps carry no units
-        int lo = 0, hi = a.batch - 1;
+        int lo = 0, hi = whole_tiles ? 0 : a.batch - 1;
         while (lo < hi) {
             const int mid = (lo + hi + 1) >> 1;
             if (pre[mid] <= w0) lo = mid; else hi = mid - 1;
         }
-        const int b = lo;
+        const int b = whole_tiles ? only : lo;
         const SeqSpan s = seq_span(a, b);
         const uint32_t nu = units_of(s.len), vl = nu + kTileCost;
-        const uint32_t in = w0 - pre[b];
+        const uint32_t in = w0 - pre[lo];
         const int h = (int)(in / vl);
         const uint32_t v0 = in - h * vl, v1 = min(vl, v0 + (w_end - w0));
         const int u0 = (int)(max(v0, kTileCost) - kTileCost), u1 = (int)(max(v1, kTileCost) - kTileCost);
@@ -652,9 +660,12 @@ cudaError_t run_step(const AttnArgs& a, cudaStream_t stream) {
     if (e != cudaSuccess) return e;
     // no more CTAs than the longest lengths the table can hold would occupy
     const int tiles = a.batch * a.pool.kv_heads, sms = device_num_sms();
-    const int64_t most = tiles * ((int64_t)a.table_width * a.pool.page_units + kTileCost);
-    const int grid = (int)std::max<int64_t>(1, std::min<int64_t>((int64_t)sms * C::CTAS, (most + kMinShare - 1) / kMinShare));
-    e = launch_attn(attn_step_kernel<D, BITS, NT>, dim3(grid), kThreads, C::SMEM, a.pdl, stream, a);
+    const int64_t units = (int64_t)a.table_width * a.pool.page_units, most = tiles * (units + kTileCost);
+    // Short tables: a CTA per tile, no join and no second launch.  Two rounds of a warp's pair of units take
+    // less than the join would.
+    if (units <= 4 * kWarps) return launch_attn(attn_step_kernel<D, BITS, NT>, dim3(tiles), kThreads, C::SMEM, a.pdl, stream, a, 1);
+    const int grid = (int)std::min<int64_t>((int64_t)sms * C::CTAS, (most + kMinShare - 1) / kMinShare);
+    e = launch_attn(attn_step_kernel<D, BITS, NT>, dim3(grid), kThreads, C::SMEM, a.pdl, stream, a, 0);
     if (e != cudaSuccess || grid == 1) return e;
     const int parts = std::max(1, std::min(4 * sms / tiles, a.max_q * a.group * (D / 64)));
     return launch_attn(attn_join_kernel<D>, dim3(tiles, parts), 256, 0, a.pdl, stream, a, grid, (int)C::ROWS);

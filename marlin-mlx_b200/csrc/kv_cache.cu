@@ -41,82 +41,93 @@ __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
 //   n = x * rsqrt(mean(x^2) + eps) * (1 + w)           (the offset weights of rms_norm)
 //   (a, b) -> (a cos - b sin, b cos + a sin)            for the rot/2 pairs of the first rot features,
 //   angle = position[axis of the pair][t] * freq        pairs (i, i + rot/2) or (2i, 2i + 1).
-// One CTA per token: the rot/2 sines and cosines are formed once in shared memory (the angle in
-// binary64 and reduced by whole turns, since a position near 10^6 leaves binary32 no fraction), then
-// dim/8 lanes take a head row, 8 features each, sums and products in binary32, one rounding at the
-// store.  The half layout's partner features sit in another lane of the same row (rot % 16 == 0), so
+// A warp takes a token's rows (or an equal share of them, where there are few tokens), 8 features per
+// lane and 32 / (dim / 8) rows at a time, the next rows' loads in flight.  The sines and cosines are formed
+// once for all its rows, spread over the lanes and handed round by shuffle: the angle in turns in binary64, since a position near
+// 10^6 leaves binary32 no fraction, its fraction in binary32.  Sums and products are binary32, rounded
+// once at the store.  The half layout's partner features sit in another lane of the row (rot % 16 == 0), so
 // they come by shuffle.
 // ------------------------------------------------------------------------------------------------
 template <int D, bool BF16_IN, bool BF16_OUT>
-__global__ void __launch_bounds__(1024) qk_norm_rope_kernel(const __grid_constant__ RopeArgs a) {
-    constexpr int LANES = D / 8;
-    __shared__ float2 cs[128];
-    const int64_t t = blockIdx.x;
-    const int tid = threadIdx.x, sub = tid & (LANES - 1);
+__global__ void __launch_bounds__(128) qk_norm_rope_kernel(const __grid_constant__ RopeArgs a, int shares) {
+    constexpr int LANES = D / 8, AT_ONCE = 32 / LANES;
+    const int lane = threadIdx.x & 31, sub = lane & (LANES - 1);
+    const uint32_t job = blockIdx.x * 4 + (threadIdx.x >> 5);
+    const int64_t t = job / shares;
+    if (t >= a.tokens) return;
+    const int rows = a.heads + a.kv_heads, half = a.rot / 2, d0 = sub * 8;
+    const int each = (rows + shares * AT_ONCE - 1) / (shares * AT_ONCE) * AT_ONCE;
+    const int from = (int)(job % shares) * each, to = min(rows, from + each);
+    auto load_row = [&](int row, float (&v)[8]) {
+        if (row >= to) return;
+        if (row >= a.heads)
+            load8(a.k, t * a.k_ts + (row - a.heads) * a.k_hs + d0, BF16_IN, v);
+        else
+            load8(a.q, t * a.q_ts + row * a.q_hs + d0, BF16_IN, v);
+    };
     pdl_wait();
     pdl_launch_dependents();
-    for (int i = tid; i < a.rot / 2; i += blockDim.x) {
-        const int ax = (a.axis[i >> 4] >> ((i & 15) * 2)) & 3;
-        const double ang = (double)a.positions[(int64_t)ax * a.tokens + t] * (double)a.freqs[i];
-        const double turns = rint(ang * 0.15915494309189535);
+    float next[8] = {};
+    load_row(from + lane / LANES, next);  // on its way while the sines are formed
+    const uint4 qw = *reinterpret_cast<const uint4*>(a.qw + d0), kw = *reinterpret_cast<const uint4*>(a.kw + d0);
+    const bool turn = d0 < a.rot, first = d0 < half;
+    // lane l forms pairs l, l + 32, ...; the pairs f0 .. f0 + 7 of a lane's features come from there (f0 is a
+    // multiple of 4 or 8, so all from one of the lanes' values)
+    float co[8], si[8];
+    const int f0 = !turn ? 0 : a.interleaved ? d0 / 2 : first ? d0 : d0 - half;
+#pragma unroll
+    for (int k = 0; k < D / 64; ++k) {
+        if (k > 0 && 32 * k >= half) break;
+        const int f = min(lane + 32 * k, half - 1), ax = (a.axis[f >> 4] >> ((f & 15) * 2)) & 3;
+        const double turns = (double)a.positions[(int64_t)ax * a.tokens + t] * ((double)a.freqs[f] * 0.15915494309189535);
         float s, c;
-        sincosf((float)fma(-turns, 6.283185307179586, ang), &s, &c);
-        cs[i] = make_float2(c, s);
-    }
-    float w[2][8];
-    load8(a.qw, sub * 8, true, w[0]);
-    load8(a.kw, sub * 8, true, w[1]);
-    __syncthreads();
-    const int rows = a.heads + a.kv_heads, half = a.rot / 2;
-    const int per_pass = blockDim.x / LANES;
-    for (int r0 = 0; r0 < rows; r0 += per_pass) {
-        const int row = r0 + tid / LANES;
-        const bool live = row < rows;
-        const bool isk = row >= a.heads;
-        const int head = isk ? row - a.heads : row;
-        float v[8] = {};
-        if (live) {
-            if (isk)
-                load8(a.k, t * a.k_ts + head * a.k_hs + sub * 8, BF16_IN, v);
-            else
-                load8(a.q, t * a.q_ts + head * a.q_hs + sub * 8, BF16_IN, v);
+        sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float x = __shfl_sync(0xffffffffu, c, (f0 + i) & 31), y = __shfl_sync(0xffffffffu, s, (f0 + i) & 31);
+            if (k == 0 || f0 >> 5 == k) {
+                co[i] = x;
+                si[i] = !a.interleaved && first ? -y : y;
+            }
         }
+    }
+    for (int r0 = from; r0 < to; r0 += AT_ONCE) {
+        const int row = r0 + lane / LANES;
+        const bool isk = row >= a.heads;
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = next[i];
+        load_row(row + AT_ONCE, next);
         float sum = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) sum = fmaf(v[i], v[i], sum);
 #pragma unroll
         for (int o = 1; o < LANES; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
         const float rs = rsqrtf(sum * (1.0f / D) + a.eps);
+        const uint32_t w[4] = {isk ? kw.x : qw.x, isk ? kw.y : qw.y, isk ? kw.z : qw.z, isk ? kw.w : qw.w};
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] *= rs * (1.0f + w[isk][i]);
-        const int d0 = sub * 8;
+        for (int i = 0; i < 4; ++i) {
+            v[2 * i] *= rs * (1.0f + __uint_as_float(w[i] << 16));
+            v[2 * i + 1] *= rs * (1.0f + __uint_as_float(w[i] & 0xffff0000u));
+        }
         if (a.interleaved) {
-            if (d0 < a.rot) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float2 e = cs[d0 / 2 + i];
-                    const float x = v[2 * i], y = v[2 * i + 1];
-                    v[2 * i] = x * e.x - y * e.y;
-                    v[2 * i + 1] = y * e.x + x * e.y;
-                }
+            for (int i = 0; i < 4 && turn; ++i) {
+                const float x = v[2 * i], y = v[2 * i + 1];
+                v[2 * i] = x * co[i] - y * si[i];
+                v[2 * i + 1] = y * co[i] + x * si[i];
             }
         } else {
-            const bool first = d0 < half, turn = d0 < a.rot;
-            const int src = (tid & 31) + (turn ? (first ? half / 8 : -half / 8) : 0);
-            float p[8];
+            const int src = lane + (turn ? (first ? half / 8 : -half / 8) : 0);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) p[i] = __shfl_sync(0xffffffffu, v[i], src);
-            if (turn) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float2 e = cs[first ? d0 + i : d0 + i - half];
-                    v[i] = v[i] * e.x + (first ? -p[i] : p[i]) * e.y;
-                }
+            for (int i = 0; i < 8; ++i) {
+                const float p = __shfl_sync(0xffffffffu, v[i], src);
+                if (turn) v[i] = v[i] * co[i] + p * si[i];
             }
         }
-        if (!live) continue;
+        if (row >= to) continue;
         void* base = isk ? a.k_out : a.q_out;
-        const int64_t o = (t * (isk ? a.kv_heads : a.heads) + head) * D + d0;
+        const int64_t o = (t * (isk ? a.kv_heads : a.heads) + (isk ? row - a.heads : row)) * D + d0;
         if (BF16_OUT) {
             *reinterpret_cast<uint4*>(static_cast<uint16_t*>(base) + o) =
                 make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
@@ -126,6 +137,20 @@ __global__ void __launch_bounds__(1024) qk_norm_rope_kernel(const __grid_constan
             y[1] = make_float4(v[4], v[5], v[6], v[7]);
         }
     }
+}
+
+// a / b correctly rounded (round to nearest even), b's reciprocal y correct to an ulp: two steps of Markstein's
+// correction, q += RN(a - b q) y, the residual exact in an FMA.  For quotients and operands well inside the
+// normal range.  __fdiv_rn, which also serves the rest, takes about four times the instructions.
+__device__ __forceinline__ float divide(float a, float b, float y) {
+    float q = a * y;
+    q = fmaf(fmaf(-b, q, a), y, q);
+    return fmaf(fmaf(-b, q, a), y, q);
+}
+__device__ __forceinline__ float reciprocal(float b) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(b));
+    return fmaf(fmaf(-b, y, 1.0f), y, y);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -138,32 +163,30 @@ __global__ void __launch_bounds__(1024) qk_norm_rope_kernel(const __grid_constan
 template <int BITS, bool BF16_IN>
 __global__ void __launch_bounds__(256) kv_write_kernel(KvPool c, const void* __restrict__ k, int64_t k_ts, int64_t k_hs,
                                                        const void* __restrict__ v, int64_t v_ts, int64_t v_hs,
-                                                       const int32_t* __restrict__ slots, int64_t items) {
+                                                       const int32_t* __restrict__ slots, int64_t tokens, int per_block) {
     pdl_wait();
     pdl_launch_dependents();
     const int lane8 = threadIdx.x & 7;
-    const int64_t item = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) >> 3;
-    const int groups = c.dim / 64, rb = c.dim * BITS / 8;
-    const bool valid = item < items;
-    // item = ((token * kv_heads + head) * 2 + value) * groups + group
-    const int64_t i2 = valid ? item / groups : 0;
-    const int g = valid ? (int)(item - i2 * groups) : 0;
-    const bool isv = i2 & 1;
-    const int64_t th = i2 >> 1, t = th / c.kv_heads;
-    const int h = (int)(th - t * c.kv_heads);
+    const int groups = c.dim / 64, rb = c.dim * BITS / 8, lg = 31 - __clz(groups);
+    // a token's items: (head * 2 + value) * groups + group
+    const int per = c.kv_heads * 2 * groups, i = blockIdx.y * 32 + (threadIdx.x >> 3), tb = i / per;
+    const int64_t t = (int64_t)blockIdx.x * per_block + tb;
+    const bool valid = t < tokens && tb < per_block;
+    const int it = i - tb * per, g = it & (groups - 1), h = it >> (lg + 1);
+    const bool isv = (it >> lg) & 1;
+    float x[8] = {};
+    if (valid) {  // not gated by the slot, whose load is still on its way
+        if (isv)
+            load8(v, t * v_ts + h * v_hs + g * 64 + lane8 * 8, BF16_IN, x);
+        else
+            load8(k, t * k_ts + h * k_hs + g * 64 + lane8 * 8, BF16_IN, x);
+    }
     const int64_t slot = valid ? slots[t] : -1;
     const int64_t unit = slot / kKvRows;
     bool put = slot >= 0;
     if (put && unit >= c.pages * c.page_units) {
         put = false;
         if (lane8 == 0) record_device_error(kDevErrBadIndex);
-    }
-    float x[8] = {};
-    if (put) {
-        if (isv)
-            load8(v, t * v_ts + h * v_hs + g * 64 + lane8 * 8, BF16_IN, x);
-        else
-            load8(k, t * k_ts + h * k_hs + g * 64 + lane8 * 8, BF16_IN, x);
     }
     float lo = INFINITY, hi = 0.0f;
 #pragma unroll
@@ -178,20 +201,46 @@ __global__ void __launch_bounds__(256) kv_write_kernel(KvPool c, const void* __r
         hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
     }
     constexpr float kTop = (float)((1 << BITS) - 1);
-    float scale = fmaxf(__fdiv_rn(__fsub_rn(hi, lo), kTop), 1e-7f);
-    const bool side = fabsf(lo) > fabsf(hi);
-    scale = side ? scale : -scale;
-    const float edge = side ? lo : hi;
-    const float steps = roundf(__fdiv_rn(edge, scale));
-    float bias = 0.0f;
-    if (steps != 0.0f) {
-        scale = __fdiv_rn(edge, steps);
-        bias = edge;
-    }
+    float scale, bias = 0.0f;
     uint32_t code[8];
+    // The group's largest magnitude decides: between 2^-20 and 2^100 every quotient below is an ordinary one
+    // (scale >= 1e-7 and >= edge / top).
+    const float most = fmaxf(fabsf(lo), fabsf(hi));
+    const bool side = fabsf(lo) > fabsf(hi);
+    const float edge = side ? lo : hi;
+    if (most > 0x1p-20f && most < 0x1p100f) {
+        scale = fmaxf(divide(__fsub_rn(hi, lo), kTop, 1.0f / kTop), 1e-7f);
+        scale = side ? scale : -scale;
+        const float steps = roundf(divide(edge, scale, reciprocal(scale)));
+        if (steps != 0.0f) {
+            scale = divide(edge, steps, reciprocal(steps));
+            bias = edge;
+        }
+        const float inv = reciprocal(scale);
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-        code[i] = (uint32_t)fminf(fmaxf(roundf(__fdiv_rn(__fsub_rn(x[i], bias), scale)), 0.0f), kTop);
+        for (int i = 0; i < 8; ++i) {
+            const float q = fminf(fmaxf(divide(__fsub_rn(x[i], bias), scale, inv), 0.0f), kTop);
+            // ties away from zero for q >= 0: floor(q + 1/2), the sum rounded down so that it passes no
+            // integer; adding 2^23, rounded down, leaves the floor in the low bits
+            code[i] = __float_as_uint(__fadd_rd(__fadd_rd(q, 0.5f), 8388608.0f)) & 255u;
+        }
+    } else {
+        scale = fmaxf(__fdiv_rn(__fsub_rn(hi, lo), kTop), 1e-7f);
+        scale = side ? scale : -scale;
+        const float steps = roundf(__fdiv_rn(edge, scale));
+        if (steps != 0.0f) {
+            scale = __fdiv_rn(edge, steps);
+            bias = edge;
+        }
+#pragma unroll 1
+        for (int i = 0; i < 8; ++i) {
+            const float v = i < 4 ? (i < 2 ? (i ? x[1] : x[0]) : (i == 2 ? x[2] : x[3])) : (i < 6 ? (i == 4 ? x[4] : x[5]) : (i == 6 ? x[6] : x[7]));
+            const uint32_t c1 = (uint32_t)fminf(fmaxf(roundf(__fdiv_rn(__fsub_rn(v, bias), scale)), 0.0f), kTop);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (j == i) code[j] = c1;
+        }
+    }
     if (!put) return;
     const int r = (int)(slot % kKvRows);
     const int64_t page = unit / c.page_units;
@@ -216,19 +265,18 @@ __global__ void __launch_bounds__(256) kv_write_kernel(KvPool c, const void* __r
 // (the operand of the attention kernels).  Rows of slots below zero read as zero, as do rows of slots
 // outside the pool, which are recorded.
 template <int BITS>
-__global__ void __launch_bounds__(256) kv_read_kernel(KvPool c, const int32_t* __restrict__ slots, int64_t items,
+__global__ void __launch_bounds__(256) kv_read_kernel(KvPool c, const int32_t* __restrict__ slots, int64_t tokens, int per_block,
                                                       uint16_t* __restrict__ ko, uint16_t* __restrict__ vo) {
     pdl_wait();
     pdl_launch_dependents();
-    const int64_t item = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    if (item >= items) return;
-    const int groups = c.dim / 64, rb = c.dim * BITS / 8, chunks = c.dim / 8;
-    // item = ((token * kv_heads + head) * 2 + value) * chunks + chunk
-    const int64_t i2 = item / chunks;
-    const int ch = (int)(item - i2 * chunks);
-    const bool isv = i2 & 1;
-    const int64_t th = i2 >> 1, t = th / c.kv_heads;
-    const int h = (int)(th - t * c.kv_heads);
+    const int groups = c.dim / 64, rb = c.dim * BITS / 8, chunks = c.dim / 8, lc = 31 - __clz(chunks);
+    // a token's items: (head * 2 + value) * chunks + chunk
+    const int per = c.kv_heads * 2 * chunks, i = blockIdx.y * 256 + threadIdx.x, tb = i / per;
+    const int64_t t = (int64_t)blockIdx.x * per_block + tb;
+    if (t >= tokens || tb >= per_block) return;
+    const int it = i - tb * per, ch = it & (chunks - 1), h = it >> (lc + 1);
+    const bool isv = (it >> lc) & 1;
+    const int64_t th = t * c.kv_heads + h;
     const int64_t slot = slots[t], unit = slot / kKvRows;
     uint4 o = make_uint4(0u, 0u, 0u, 0u);
     if (slot >= 0 && unit < c.pages * c.page_units) {
@@ -261,9 +309,9 @@ __global__ void __launch_bounds__(256) kv_read_kernel(KvPool c, const int32_t* _
 }
 
 template <typename... P, typename... A>
-cudaError_t launch_pdl(void (*kernel)(P...), int64_t blocks, int threads, bool pdl, cudaStream_t stream, A... args) {
+cudaError_t launch_pdl(void (*kernel)(P...), dim3 grid, int threads, bool pdl, cudaStream_t stream, A... args) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)blocks);
+    cfg.gridDim = grid;
     cfg.blockDim = dim3(threads);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
@@ -274,33 +322,43 @@ cudaError_t launch_pdl(void (*kernel)(P...), int64_t blocks, int threads, bool p
     return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
 }
 
+// 256-thread blocks over tokens of `lanes` threads each: several tokens per block, or several blocks (y) per
+// token.  Keeps the split of an index into token, head and group in 32 bits.
+inline dim3 token_grid(int lanes, int64_t tokens, int& per_block) {
+    per_block = std::max(1, 256 / lanes);
+    return dim3((unsigned)((tokens + per_block - 1) / per_block), (unsigned)((lanes * per_block + 255) / 256));
+}
+
 template <int D>
-cudaError_t rope_dim(const RopeArgs& a, bool bi, bool bo, int64_t blocks, int threads, bool pdl, cudaStream_t s) {
-    if (bi && bo) return launch_pdl(qk_norm_rope_kernel<D, true, true>, blocks, threads, pdl, s, a);
-    if (bi) return launch_pdl(qk_norm_rope_kernel<D, true, false>, blocks, threads, pdl, s, a);
-    if (bo) return launch_pdl(qk_norm_rope_kernel<D, false, true>, blocks, threads, pdl, s, a);
-    return launch_pdl(qk_norm_rope_kernel<D, false, false>, blocks, threads, pdl, s, a);
+cudaError_t rope_dim(const RopeArgs& a, bool bi, bool bo, bool pdl, cudaStream_t s) {
+    // Warps per token: about 32 per SM over all tokens, each at least one pass of rows.  A share repeats the
+    // sines, so no more than that.
+    const int passes = ((a.heads + a.kv_heads) * (D / 8) + 31) / 32;
+    const int64_t want = (32 * device_num_sms() + a.tokens - 1) / a.tokens;
+    const int shares = (int)std::min<int64_t>(passes, std::max<int64_t>(1, want));
+    const dim3 blocks((unsigned)((a.tokens * shares + 3) / 4));
+    if (bi && bo) return launch_pdl(qk_norm_rope_kernel<D, true, true>, blocks, 128, pdl, s, a, shares);
+    if (bi) return launch_pdl(qk_norm_rope_kernel<D, true, false>, blocks, 128, pdl, s, a, shares);
+    if (bo) return launch_pdl(qk_norm_rope_kernel<D, false, true>, blocks, 128, pdl, s, a, shares);
+    return launch_pdl(qk_norm_rope_kernel<D, false, false>, blocks, 128, pdl, s, a, shares);
 }
 
 }  // namespace
 
 cudaError_t launch_qk_norm_rope(const RopeArgs& a, int dtype, int out_dtype, bool pdl, cudaStream_t stream) {
-    // few tokens: the whole token in one pass of its CTA; many: smaller CTAs, several per SM
-    const int lanes = (a.heads + a.kv_heads) * (a.dim / 8);
-    const int most = a.tokens <= 2 * device_num_sms() ? 1024 : 256;
-    const int threads = std::min(most, (lanes + 31) / 32 * 32);
     const bool bi = dtype == kDtypeBF16, bo = out_dtype == kDtypeBF16;
-    if (a.dim == 64) return rope_dim<64>(a, bi, bo, a.tokens, threads, pdl, stream);
-    if (a.dim == 128) return rope_dim<128>(a, bi, bo, a.tokens, threads, pdl, stream);
-    return rope_dim<256>(a, bi, bo, a.tokens, threads, pdl, stream);
+    if (a.dim == 64) return rope_dim<64>(a, bi, bo, pdl, stream);
+    if (a.dim == 128) return rope_dim<128>(a, bi, bo, pdl, stream);
+    return rope_dim<256>(a, bi, bo, pdl, stream);
 }
 
 cudaError_t launch_kv_write(const KvPool& c, const void* k, int64_t k_ts, int64_t k_hs, const void* v, int64_t v_ts,
                             int64_t v_hs, int dtype, const int32_t* slots, int64_t tokens, bool pdl, cudaStream_t stream) {
-    const int64_t items = tokens * c.kv_heads * 2 * (c.dim / 64), blocks = (items * 8 + 255) / 256;
+    int tb;
+    const dim3 grid = token_grid(c.kv_heads * 2 * (c.dim / 64) * 8, tokens, tb);
     const bool b = dtype == kDtypeBF16;
     auto go = [&](auto kernel) {
-        return launch_pdl(kernel, blocks, 256, pdl, stream, c, k, k_ts, k_hs, v, v_ts, v_hs, slots, items);
+        return launch_pdl(kernel, grid, 256, pdl, stream, c, k, k_ts, k_hs, v, v_ts, v_hs, slots, tokens, tb);
     };
     if (c.bits == 4) return b ? go(kv_write_kernel<4, true>) : go(kv_write_kernel<4, false>);
     return b ? go(kv_write_kernel<8, true>) : go(kv_write_kernel<8, false>);
@@ -308,9 +366,10 @@ cudaError_t launch_kv_write(const KvPool& c, const void* k, int64_t k_ts, int64_
 
 cudaError_t launch_kv_read(const KvPool& c, const int32_t* slots, int64_t tokens, uint16_t* k, uint16_t* v, bool pdl,
                            cudaStream_t stream) {
-    const int64_t items = tokens * c.kv_heads * 2 * (c.dim / 8), blocks = (items + 255) / 256;
-    if (c.bits == 4) return launch_pdl(kv_read_kernel<4>, blocks, 256, pdl, stream, c, slots, items, k, v);
-    return launch_pdl(kv_read_kernel<8>, blocks, 256, pdl, stream, c, slots, items, k, v);
+    int tb;
+    const dim3 grid = token_grid(c.kv_heads * 2 * (c.dim / 8), tokens, tb);
+    if (c.bits == 4) return launch_pdl(kv_read_kernel<4>, grid, 256, pdl, stream, c, slots, tokens, tb, k, v);
+    return launch_pdl(kv_read_kernel<8>, grid, 256, pdl, stream, c, slots, tokens, tb, k, v);
 }
 
 int kv_device_error(bool clear) { return tu_device_error(clear); }

@@ -20,41 +20,49 @@ from ._lib import BF16, F32, KvCache, check
 _CODES = {torch.bfloat16: BF16, torch.float32: F32}
 
 
-def _same_device(first: torch.Tensor, **others: torch.Tensor | None) -> None:
-    if not first.is_cuda:
+def _device(first: torch.Tensor, *others: torch.Tensor | None) -> int:
+    """The CUDA device all of them are on."""
+    d = first.get_device()
+    if d < 0:
         raise ValueError("expected CUDA tensors")
-    for name, t in others.items():
-        if t is not None and t.device != first.device:
-            raise ValueError(f"{name} is on {t.device}, expected {first.device}")
+    for t in others:
+        if t is not None and t.get_device() != d:
+            raise ValueError(f"tensors on different devices: {first.device} and {t.device}")
+    return d
 
 
-def _on(t: torch.Tensor):
-    """Makes t's device the current one for the call, where it is not already."""
-    if t.device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(t.device)
+def _current(device: int):
+    """Makes the device the current one, where it is not already."""
+    return contextlib.nullcontext() if device == torch.cuda.current_device() else torch.cuda.device(device)
 
 
-def _stream(t: torch.Tensor) -> int:
-    return torch.cuda.current_stream(t.device).cuda_stream
+def _call(device: int, name: str, *args) -> None:
+    """Calls the library on the device's current stream (its last argument), with the device current."""
+    fn = getattr(_lib.load(), name)
+    stream = torch._C._cuda_getCurrentRawStream(device)
+    with _current(device):
+        status = fn(*args, stream)
+    if status:
+        check(status, name)
 
 
-def _heads(t: torch.Tensor, name: str) -> torch.Tensor:
+def _heads(t: torch.Tensor, name: str):
+    """Shape and strides of a [tokens, heads, head_dim] operand."""
     if t.dim() != 3:
         raise ValueError(f"{name} must be [tokens, heads, head_dim], got {tuple(t.shape)}")
     if t.dtype not in _CODES:
         raise TypeError(f"{name} must be bfloat16 or float32, got {t.dtype}")
-    if t.stride(2) != 1 and t.shape[2] > 1:
+    stride = t.stride()
+    if stride[2] != 1:
         raise ValueError(f"{name}'s features must be contiguous")
-    return t
+    return t.shape, stride
 
 
-def _int32(t: torch.Tensor, name: str, *shape: int) -> torch.Tensor:
-    if t.dtype != torch.int32:
+def _int32(t: torch.Tensor, name: str, *shape: int) -> None:
+    if t.dtype is not torch.int32:
         raise TypeError(f"{name} must be int32, got {t.dtype}")
-    if tuple(t.shape) != shape or not t.is_contiguous():
+    if t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous {list(shape)}, got {list(t.shape)}")
-    return t
 
 
 class KVCache:
@@ -70,6 +78,7 @@ class KVCache:
         self.data, self.head_dim, self.bits = data, head_dim, bits
         self.pages, self.kv_heads, self.page_size = data.shape[0], data.shape[1], data.shape[2] * 16
         self._c = KvCache(data.data_ptr(), self.pages, self.page_size, self.kv_heads, head_dim, bits)
+        self._ref = ctypes.byref(self._c)
 
     @classmethod
     def empty(cls, pages: int, page_size: int, kv_heads: int, head_dim: int, bits: int = 4,
@@ -102,57 +111,50 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_wei
 
     q [tokens, heads, head_dim] and k [tokens, kv_heads, head_dim], bf16 or f32, may be strided views of a
     fused projection; positions int32 [tokens] or [axes, tokens].  Returns contiguous (q, k) of out_dtype."""
-    _heads(q, "q"), _heads(k, "k")
+    (t, h, d), qs = _heads(q, "q")
+    kshape, ks = _heads(k, "k")
     if q.dtype != k.dtype or out_dtype not in _CODES:
         raise TypeError("q and k must have one dtype, out_dtype must be bfloat16 or float32")
-    t, h, d = q.shape
-    if k.shape[0] != t or k.shape[2] != d:
+    kvh = kshape[1]
+    if kshape[0] != t or kshape[2] != d:
         raise ValueError(f"k {tuple(k.shape)} does not match q {tuple(q.shape)}")
-    if positions.dim() == 1:
-        positions = positions[None]
-    _int32(positions, "positions", positions.shape[0], t)
+    axes = 1 if positions.dim() == 1 else positions.shape[0]
+    _int32(positions, "positions", *((t,) if positions.dim() == 1 else (axes, t)))
     for w, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
-        if w.dtype != torch.bfloat16 or tuple(w.shape) != (d,) or not w.is_contiguous():
+        if w.dtype is not torch.bfloat16 or w.shape != (d,) or not w.is_contiguous():
             raise ValueError(f"{name} must be contiguous bfloat16 [{d}]")
-    _same_device(q, k=k, q_weight=q_weight, k_weight=k_weight, positions=positions, inv_freq=rotary.inv_freq)
-    qo = torch.empty((t, h, d), dtype=out_dtype, device=q.device)
-    ko = torch.empty((t, k.shape[1], d), dtype=out_dtype, device=q.device)
-    with _on(q):
-        check(_lib.load().marlin_q4_qk_norm_rope(
-            q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), _CODES[q.dtype], t, h,
-            k.shape[1], d, q_weight.data_ptr(), k_weight.data_ptr(), eps, positions.data_ptr(), positions.shape[0],
-            rotary.axes, rotary.inv_freq.data_ptr(), 2 * rotary.inv_freq.numel(), int(rotary.interleaved),
-            qo.data_ptr(), ko.data_ptr(), _CODES[out_dtype], _stream(q)), "marlin_q4_qk_norm_rope")
+    dev = _device(q, k, q_weight, k_weight, positions, rotary.inv_freq)
+    qo = q.new_empty((t, h, d), dtype=out_dtype)
+    ko = q.new_empty((t, kvh, d), dtype=out_dtype)
+    _call(dev, "marlin_q4_qk_norm_rope", q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], _CODES[q.dtype], t, h, kvh, d,
+          q_weight.data_ptr(), k_weight.data_ptr(), eps, positions.data_ptr(), axes, rotary.axes, rotary.inv_freq.data_ptr(),
+          2 * rotary.inv_freq.shape[0], rotary.interleaved, qo.data_ptr(), ko.data_ptr(), _CODES[out_dtype])
     return qo, ko
 
 
 def kv_write(cache: KVCache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
     """Quantize k, v [tokens, kv_heads, head_dim] (bf16 or f32) into the cache rows ``slots`` (int32
     [tokens], page * page_size + row; negative: skip the token).  The slots >= 0 must differ."""
-    _heads(k, "k"), _heads(v, "v")
-    t = k.shape[0]
-    if tuple(k.shape) != (t, cache.kv_heads, cache.head_dim) or k.shape != v.shape or k.dtype != v.dtype:
+    (t, h, d), ks = _heads(k, "k")
+    _, vs = _heads(v, "v")
+    if h != cache.kv_heads or d != cache.head_dim or k.shape != v.shape or k.dtype != v.dtype:
         raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} must be [tokens, {cache.kv_heads}, {cache.head_dim}]"
                          " of one dtype")
     _int32(slots, "slots", t)
-    _same_device(cache.data, k=k, v=v, slots=slots)
-    with _on(k):
-        check(_lib.load().marlin_q4_kv_write(ctypes.byref(cache._c), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(),
-                                             v.stride(0), v.stride(1), _CODES[k.dtype], slots.data_ptr(), t, _stream(k)),
-              "marlin_q4_kv_write")
+    dev = _device(cache.data, k, v, slots)
+    _call(dev, "marlin_q4_kv_write", cache._ref, k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], _CODES[k.dtype],
+          slots.data_ptr(), t)
 
 
 def kv_read(cache: KVCache, slots: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """The keys and values of cache rows ``slots`` (int32 [tokens]; negative: zeros) as bf16 [tokens,
     kv_heads, head_dim], bf16(scale * code + bias)."""
-    _int32(slots, "slots", *slots.shape[:1])
-    _same_device(cache.data, slots=slots)
-    shape = (slots.numel(), cache.kv_heads, cache.head_dim)
-    k = torch.empty(shape, dtype=torch.bfloat16, device=slots.device)
-    v = torch.empty(shape, dtype=torch.bfloat16, device=slots.device)
-    with _on(slots):
-        check(_lib.load().marlin_q4_kv_read(ctypes.byref(cache._c), slots.data_ptr(), slots.numel(), k.data_ptr(),
-                                            v.data_ptr(), _stream(slots)), "marlin_q4_kv_read")
+    t = slots.numel()
+    _int32(slots, "slots", t)
+    dev = _device(cache.data, slots)
+    k = slots.new_empty((t, cache.kv_heads, cache.head_dim), dtype=torch.bfloat16)
+    v = slots.new_empty((t, cache.kv_heads, cache.head_dim), dtype=torch.bfloat16)
+    _call(dev, "marlin_q4_kv_read", cache._ref, slots.data_ptr(), t, k.data_ptr(), v.data_ptr())
     return k, v
 
 
@@ -166,33 +168,32 @@ def paged_attention(q: torch.Tensor, cache: KVCache, block_table: torch.Tensor, 
     any, or None for one token per sequence.  scale defaults to head_dim ** -0.5.  Rows of ``out`` outside
     every sequence are left as they were.  workspace: uint8 of at least attention_workspace_size bytes; calls
     that may overlap in time (other streams, graphs) need one each.  Without it one is allocated."""
-    _heads(q, "q")
-    if q.dtype != torch.bfloat16:
+    (t, h, d), qs = _heads(q, "q")
+    if q.dtype is not torch.bfloat16:
         raise TypeError(f"q must be bfloat16, got {q.dtype}")
-    t, h, d = q.shape
     if d != cache.head_dim:
         raise ValueError(f"q's head_dim {d} is not the cache's {cache.head_dim}")
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or (block_table.shape[1] > 1 and block_table.stride(1) != 1):
-        raise ValueError("block_table must be int32 [batch, pages] with contiguous rows")
-    batch = block_table.shape[0]
+    if block_table.dtype is not torch.int32 or block_table.dim() != 2:
+        raise ValueError("block_table must be int32 [batch, pages]")
+    batch, width = block_table.shape
+    ts = block_table.stride()
+    if ts[1] != 1 and width > 1:
+        raise ValueError("block_table's rows must be contiguous")
     _int32(kv_lens, "kv_lens", batch)
     if cu_q is not None:
         _int32(cu_q, "cu_q", batch + 1)
-    _same_device(q, cache=cache.data, block_table=block_table, kv_lens=kv_lens, cu_q=cu_q, out=out, workspace=workspace)
+    dev = _device(q, cache.data, block_table, kv_lens, cu_q, out, workspace)
     if out is None:
-        out = torch.empty((t, h, d), dtype=torch.bfloat16, device=q.device)
-    elif out.dtype != torch.bfloat16 or out.shape != q.shape or not out.is_contiguous():
+        out = q.new_empty((t, h, d))
+    elif out.dtype is not torch.bfloat16 or out.shape != q.shape or not out.is_contiguous():
         raise ValueError(f"out must be contiguous bfloat16 {list(q.shape)}")
-    lib = _lib.load()
-    with _on(q):
-        if workspace is None:
-            size = lib.marlin_q4_paged_attention_workspace_size(t, h, cache.kv_heads, d, max(batch, 1))
-            workspace = torch.empty(size, dtype=torch.uint8, device=q.device)
-        check(lib.marlin_q4_paged_attention(
-            q.data_ptr(), q.stride(0), q.stride(1), ctypes.byref(cache._c), t, h, block_table.data_ptr(),
-            block_table.stride(0), block_table.shape[1], kv_lens.data_ptr(),
-            None if cu_q is None else cu_q.data_ptr(), batch, max_q, d ** -0.5 if scale is None else scale,
-            out.data_ptr(), workspace.data_ptr(), workspace.numel(), _stream(q)), "marlin_q4_paged_attention")
+    if workspace is None:
+        with _current(dev):
+            size = _lib.load().marlin_q4_paged_attention_workspace_size(t, h, cache.kv_heads, d, max(batch, 1))
+        workspace = q.new_empty(size, dtype=torch.uint8)
+    _call(dev, "marlin_q4_paged_attention", q.data_ptr(), qs[0], qs[1], cache._ref, t, h, block_table.data_ptr(), ts[0], width,
+          kv_lens.data_ptr(), None if cu_q is None else cu_q.data_ptr(), batch, max_q, d ** -0.5 if scale is None else scale,
+          out.data_ptr(), workspace.data_ptr(), workspace.numel())
     return out
 
 

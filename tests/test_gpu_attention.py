@@ -188,6 +188,35 @@ def test_four_bit_rows_are_quantize_weight():
         assert np.array_equal(f64(y), want)
 
 
+def test_many_groups_are_quantize_weight():
+    """A million groups over all binary orders of magnitude, ties and equal values among them: the cache's own
+    division gives the codes of quantize_weight (which divides by __fdiv_rn) every time."""
+    g = torch.Generator(device=DEV).manual_seed(5)
+    n = 1 << 18
+    x = torch.randn((n, 4, 64), generator=g, device=DEV)
+    x = x * torch.exp2(torch.randint(-40, 40, (n, 4, 1), generator=g, device=DEV).float())
+    x[::7] = torch.randint(-20, 20, x[::7].shape, generator=g, device=DEV).float()  # quotients that tie
+    x[::31] = x[::31].abs()
+    x[::37] *= 2.0**-100
+    x[::41] *= 2.0**80
+    x = x.bfloat16().reshape(n, 1, 256)
+    cache = mq.KVCache.empty(n // 1024, 1024, 1, 256, 4)
+    slots = torch.arange(n, dtype=torch.int32, device=DEV)
+    mq.kv_write(cache, x, x, slots)
+    q = mq.quantize_weight(x.reshape(n, 256))
+    codes = (q.weight[..., None] >> (4 * torch.arange(8, device=DEV)) & 15).reshape(n, 4, 64)
+    want = (codes.double() * q.scales.double()[..., None] + q.biases.double()[..., None]).reshape(n, 1, 256)
+    for y in mq.kv_read(cache, slots):
+        assert torch.equal(y, want.bfloat16())  # double products and sums are exact, one rounding
+    # 8 bits: the codes differ from the exact quotient's only where it ties
+    cache = mq.KVCache.empty(n // 1024, 1024, 1, 256, 8)
+    mq.kv_write(cache, x, x, slots)
+    sample = torch.randint(0, n, (4096,), generator=g, device=DEV)
+    k, _ = mq.kv_read(cache, sample.int())
+    c, s, b = ref.quantize(f64(x[sample]), 8)
+    assert np.array_equal(f64(k), ref.bf16(ref.dequantize(c, s, b)))
+
+
 def test_slots_outside_the_pool_are_refused_on_the_device():
     cache = mq.KVCache.empty(2, 16, 1, 64, 8)
     x = rand((4, 1, 64), 1)
