@@ -7,16 +7,18 @@
 //   P = 2^(c S - M + e)         one thread per row, written back over S as f16
 //   O[128 x dim] += P V         P from TMEM, V in shared memory (features contiguous: an MN-major operand)
 // Keys and values are dequantized to f16 (11 bits, one rounding of scale * code + bias) rather than bf16:
-// the tile's largest bias gives a power of two that puts them in range, 2^eK for a step's keys, folded into
-// the softmax factor c, 2^e for its values, folded into the exponent; M is the running maximum of
-// (c S + e), so a step with small values never loses its weights' bits.  Each query row is scaled by its own
-// power of two.  M moves only when a row outgrows it by 2^8, which keeps the rescaling of O rare.
+// the largest bias of a unit of 16 positions gives a power of two that puts it in range, 2^eK for its keys,
+// folded into the softmax factor c of its columns, 2^e for its values, folded into their exponent; M is the
+// running maximum of (c S + e), so a unit with small values never loses its weights' bits.  Each query row
+// is scaled by its own power of two.  M moves only when a row outgrows it by 2^8, which keeps the rescaling
+// of O rare.
 //
 // Bound: tensor pipe (dim 256: 2048 cycles a step), the exponentials (128 x 128 at 16 a cycle and SM: 1024)
 // or the issue slots of dequantizing (about 2 instructions per cached value and tile).
-// Warps: 0-3 softmax and output, 4 issues the MMAs, 5-12 dequantize (codes prefetched to registers one step
-// ahead, straight from the pages).  Items (tile, range of steps) are laid out by a planning kernel from the
-// lengths on the device: no more steps per item than an SM's fair share, longest tiles first, taken by
+// Warps: 0-7 softmax and output (two threads per row, 64 columns each, who agree on M through shared
+// memory), the next 4 or 8 dequantize, each its own units, codes prefetched to registers one step ahead
+// straight from the pages, and one issues the MMAs.  Items (tile, range of steps) are laid out by a planning kernel from
+// the lengths on the device: no more steps per item than an SM's fair share, longest tiles first, taken by
 // persistent CTAs from a counter; a tile of several items is joined from binary32 partial rows in item order.
 #include <algorithm>
 
@@ -28,10 +30,8 @@ namespace {
 
 constexpr int kRows = 128;       // rows of a tile (M)
 constexpr int kKeys = 128;       // positions of a step
-constexpr int kSoft = 4;         // softmax warps
-constexpr int kWarpMma = 4;
-constexpr int kDeq = 8;          // dequantizing warps, from warp 5
-constexpr int kThreads = (kSoft + 1 + kDeq) * 32;
+constexpr int kSoft = 8;         // softmax warps
+constexpr int kWarpDeq = 8;      // first dequantizing warp
 constexpr int kItemCost = 2;     // fixed cost of an item (queries, pipeline fill, output), in steps
 constexpr uint32_t kTmemCols = 512;
 constexpr float kLazy = 8.f;     // log2 of how far a row may outgrow its maximum before O is rescaled
@@ -180,11 +180,24 @@ struct ChunkCfg {
     static constexpr int RB = kv_row_bytes(D, BITS), G = D / 64, UB = kv_unit_bytes(D, BITS);
     static constexpr int NB = D == 256 ? 1 : 2;           // dequantized K and V buffers
     static constexpr int SB = D == 256 ? 2 : 3;           // S buffers in TMEM (128 columns each, O behind them)
-    static constexpr int KC = RB / 32;                    // 16-byte pieces per dequantizing thread and step
+    static constexpr int DW = 8;                          // dequantizing warps
+    static constexpr int UPW = 8 / DW;                    // units of a step per dequantizing warp
+    static constexpr int KC = RB / 32;                    // 16-byte pieces per lane and unit
+    // 8-bit codes of many features would take 64 registers for a step: V follows K through the same ones
+    static constexpr bool ONE = D == 256 && BITS == 8;
+    // Warpgroups: two softmax, one or two dequantizing, and one whose first warp issues the MMAs.  The issuer
+    // hands its registers to the others (the launch's total: 512 x 128 or 640 x 96).
+    static constexpr int WARP_MMA = kWarpDeq + DW, THREADS = (WARP_MMA + 4) * 32;
+    static constexpr int REGS_SOFT = D == 256 ? 112 : 128, REGS_DEQ = D == 256 ? 112 : 96, REGS_MMA = 24;
+    static constexpr int REGS_ALL = (kSoft * REGS_SOFT + DW * REGS_DEQ + 4 * REGS_MMA) * 32;
+    static_assert(REGS_ALL <= THREADS * 96);
     static constexpr uint32_t QB = kRows * D * 2, KB = kKeys * D * 2;
     static constexpr uint32_t OFF_K = QB, OFF_V = OFF_K + NB * KB, OFF_T = OFF_V + NB * KB;
-    static constexpr uint32_t TAB = 2 * G * kKeys * 4;    // f16 (scale, bias) of a step: [K, V][group][position]
-    static constexpr uint32_t OFF_SR = OFF_T + 2 * TAB;
+    static constexpr uint32_t TAB = 2 * 8 * 2 * G * 16 * 4;  // f16 (scale, bias): [2 steps][unit][K, V][group][row]
+    static constexpr bool KEEP = D <= 128;                // a softmax thread keeps its 64 scores in registers
+    static constexpr uint32_t OFF_E = OFF_T + TAB;        // exponents [4 steps][unit]: 2^eK, e, 2^-e
+    static constexpr uint32_t OFF_X = OFF_E + 4 * 8 * 16; // [2 steps][half][row]: maxima of the two halves of a row
+    static constexpr uint32_t OFF_SR = OFF_X + 2 * 2 * kRows * 4;
     static constexpr uint32_t OFF_BAR = OFF_SR + kRows * 4;
     static constexpr uint32_t SMEM = 1024 + OFF_BAR + 256;
 };
@@ -216,7 +229,8 @@ __device__ __forceinline__ uint64_t umma_desc_mn_sw128(const void* smem_ptr, uin
 }
 constexpr uint32_t kIdescBMn = 1u << 16;  // B is MN-major
 
-__device__ __forceinline__ void deq_barrier() { asm volatile("bar.sync 1, %0;" ::"n"(kDeq * 32) : "memory"); }
+// the two warps of a TMEM lane quarter
+__device__ __forceinline__ void pair_barrier(int quarter) { asm volatile("bar.sync %0, 64;" ::"r"(quarter + 1) : "memory"); }
 
 __device__ __forceinline__ uint32_t f16x2_fma(uint32_t a, uint32_t b, uint32_t c) {
     uint32_t d;
@@ -261,16 +275,44 @@ __device__ __forceinline__ void dequant_piece(const uint4& x, uint32_t pair, uin
     }
 }
 
+// two binary32 at once
+__device__ __forceinline__ uint64_t f32x2(float lo, float hi) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
+    return d;
+}
+__device__ __forceinline__ void f32x2_split(uint64_t v, float& lo, float& hi) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t f32x2_fma(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t f32x2_add(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+
+template <int REGS>
+__device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS)); }
+template <int REGS>
+__device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS)); }
+
 template <int D, int BITS>
-__global__ void __launch_bounds__(kThreads, 1) attn_chunk_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ ChunkWork work) {
+__global__ void __launch_bounds__(ChunkCfg<D, BITS>::THREADS, 1)
+    attn_chunk_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ ChunkWork work) {
     using C = ChunkCfg<D, BITS>;
-    constexpr int G = C::G, NB = C::NB, SB = C::SB, KC = C::KC;
+    constexpr int G = C::G, NB = C::NB, SB = C::SB, KC = C::KC, DW = C::DW, UPW = C::UPW, kWarpMma = C::WARP_MMA;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = align_smem_1024(smem_raw);
     uint8_t* sq = smem;
     uint8_t* sk = smem + C::OFF_K;
     uint8_t* sv = smem + C::OFF_V;
     uint32_t* tab = reinterpret_cast<uint32_t*>(smem + C::OFF_T);
+    float4* expo = reinterpret_cast<float4*>(smem + C::OFF_E);
+    float* xch = reinterpret_cast<float*>(smem + C::OFF_X);
     float* qsr = reinterpret_cast<float*>(smem + C::OFF_SR);
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
     uint64_t* kfull = bars;            // [NB] dequantizing warps
@@ -281,11 +323,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_chunk_kernel(const __grid_co
     uint64_t* pfull = sfull + SB;      // [SB] softmax warps
     uint64_t* efull = pfull + SB;      // [4] dequantizing warps: the step's exponents (they run up to 3 steps ahead)
     uint64_t* pdone = efull + 4;       // [SB] MMA commit: P V of the step (and of all before it) done
-    uint64_t* fin = pdone + SB;         // [1]
+    uint64_t* fin = pdone + SB;        // [1]
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_s, item_s;
-    __shared__ uint32_t emax[4][2];
-    __shared__ float expo[4][2];       // 2^eK, eV of a step
     volatile int* abort = &abort_s;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
@@ -296,9 +336,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_chunk_kernel(const __grid_co
     if (tid == 0) {
         abort_s = 0;
         for (int i = 0; i < NB; ++i) {
-            mbar_init(&kfull[i], kDeq);
+            mbar_init(&kfull[i], DW);
             mbar_init(&kfree[i], 1);
-            mbar_init(&vfull[i], kDeq);
+            mbar_init(&vfull[i], DW);
             mbar_init(&vfree[i], 1);
         }
         for (int i = 0; i < SB; ++i) {
@@ -306,11 +346,10 @@ __global__ void __launch_bounds__(kThreads, 1) attn_chunk_kernel(const __grid_co
             mbar_init(&pdone[i], 1);
             mbar_init(&pfull[i], kSoft);
         }
-        for (int i = 0; i < 4; ++i) mbar_init(&efull[i], kDeq);
+        for (int i = 0; i < 4; ++i) mbar_init(&efull[i], DW);
         mbar_init(fin, 1);
         fence_mbar_init();
     }
-    if (tid < 8) emax[tid >> 1][tid & 1] = 0u;
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -319,147 +358,419 @@ __global__ void __launch_bounds__(kThreads, 1) attn_chunk_kernel(const __grid_co
     pdl_launch_dependents();
     const int total = work.head[1] * a.pool.kv_heads;
 
-    uint32_t base = 0;  // steps of the CTA's earlier items (barrier phases run on)
-    for (;;) {
-        if (tid == 0) item_s = *abort ? total : atomicAdd(&work.head[0], 1);
-        __syncthreads();
-        const int id = item_s;
-        if (id >= total) break;
-        const Item it = work.items[id / a.pool.kv_heads];
-        const int h = id % a.pool.kv_heads;
-        const SeqSpan s = seq_span(a, it.b);
-        const int n = it.k1 - it.k0;
-        const int nrows = min(kRows, s.n * a.group - it.row0);
-        const int nu = (s.len + kKvRows - 1) / kKvRows;
-
-        // dequantizing warps: the codes of the first step on their way before anything else
-        const int dw = warp - 5;
-        uint4 kr[KC], vr[KC];
-        uint32_t pr[G];
-        const uint8_t* ua = nullptr;  // unit (lane & 7) of the step whose loads come next
-        int page = 0;                 // its table entry, read a step earlier
-        auto fetch_page = [&](int j) {
-            const int u = min((it.k0 + j) * 8 + (lane & 7), nu - 1);
-            page = table_page(a, it.b, u / a.pool.page_units);
-        };
-        auto unit_at = [&](int j) {
-            const int u = min((it.k0 + j) * 8 + (lane & 7), nu - 1);
-            ua = a.pool.data + (((int64_t)page * a.pool.kv_heads + h) * a.pool.page_units + u % a.pool.page_units) * (int64_t)C::UB;
-        };
-        auto unit_ptr = [&](int u) { return reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(ua), u)); };
-        auto load_pr = [&]() {  // this thread's position (tid mod 128) of K (first 128 threads) or V
-            const int key = (dw & 3) * 32 + lane;
-            const uint64_t lo = reinterpret_cast<uint64_t>(ua);
-            const uint8_t* p0 = reinterpret_cast<const uint8_t*>(__shfl_sync(0xffffffffu, lo, key >> 4));
-            const uint8_t* p = p0 + (dw < 4 ? kv_key_pair(key & 15, 0, C::RB, G) : kv_value_pair(key & 15, 0, C::RB, G));
-            if constexpr (G == 4) {
-                const uint4 x = __ldg(reinterpret_cast<const uint4*>(p));
-                pr[0] = x.x, pr[1] = x.y, pr[2] = x.z, pr[3] = x.w;
-            } else if constexpr (G == 2) {
-                const uint2 x = __ldg(reinterpret_cast<const uint2*>(p));
-                pr[0] = x.x, pr[1] = x.y;
-            } else {
-                pr[0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+    // Every warp meets the others three times an item: number known, queries in place, item done.
+    auto sync_all = [] { asm volatile("bar.sync 0, %0;" ::"n"(C::THREADS) : "memory"); };
+    // Queries, by all but the last warpgroup: D / 8 lanes per row, scaled by a power of two to a maximum in [2^10, 2^11)
+    auto load_queries = [&](const Item& it, const SeqSpan& s, int h, int nrows) {
+        constexpr int LPR = D / 8, RPW = 32 / LPR;
+        for (int r0 = warp * RPW; r0 < kRows; r0 += (kSoft + DW) * RPW) {
+            const int r = r0 + lane / LPR, c = lane % LPR;
+            uint4 x = make_uint4(0u, 0u, 0u, 0u);
+            if (r < nrows) {
+                const int rr = it.row0 + r;
+                x = *reinterpret_cast<const uint4*>(a.q + (int64_t)(s.q0 + rr / a.group) * a.q_ts +
+                                                    (int64_t)(h * a.group + rr % a.group) * a.q_hs + c * 8);
             }
-        };
-        auto load_k = [&]() {
-#pragma unroll
-            for (int i = 0; i < KC; ++i) {
-                const int blk = dw + 8 * i;
-                if (C::RB >= 64) {  // 8 rows x one 64-byte panel
-                    const int rowblk = blk & 15, panel = blk >> 4;
-                    const uint8_t* u = unit_ptr(rowblk >> 1);
-                    kr[i] = __ldg(reinterpret_cast<const uint4*>(u + panel * 1024 + ((rowblk & 1) * 8 + (lane & 7)) * 64 + (lane >> 3) * 16));
-                } else {            // 16 rows x 32 bytes
-                    const uint8_t* u = unit_ptr(blk);
-                    kr[i] = __ldg(reinterpret_cast<const uint4*>(u + ((lane & 7) + 8 * (lane >> 4)) * 32 + ((lane >> 3) & 1) * 16));
-                }
-            }
-        };
-        auto load_v = [&]() {
-#pragma unroll
-            for (int i = 0; i < KC; ++i) {  // 512 bytes: two pieces of each of a unit's 16 rows
-                const int blk = dw + 8 * i, u8 = blk & 7, pair = blk >> 3;
-                const uint8_t* u = unit_ptr(u8);
-                vr[i] = __ldg(reinterpret_cast<const uint4*>(u + kKvRows * (C::RB + 4 * G) + pair * 512 + (lane >> 4) * 256 +
-                                                             ((lane >> 2) & 1) * 128 + ((lane >> 3) & 1) * 64 + (lane & 3) * 16));
-            }
-        };
-        // exponents and f16 (scale, bias) of step j from pr, in two parts around a barrier
-        auto prep_max = [&](int j) {
-            const int key = (dw & 3) * 32 + lane;
+            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
             uint32_t big = 0;
 #pragma unroll
-            for (int i = 0; i < G; ++i) {
-                if ((it.k0 + j) * kKeys + key >= s.len) pr[i] = 0u;  // behind the last position: zeros
-                const uint32_t sc = pr[i] & 0x7fffu, bi = (pr[i] >> 16) & 0x7fffu;
-                // |value| <= max(|bias|, 16 or 256 |scale|) up to a factor of two
-                big = max(big, max(bi, sc ? sc + (BITS << 7) : 0u));
-            }
-            big = __reduce_max_sync(0xffffffffu, big);
-            if (lane == 0) atomicMax(&emax[(base + j) & 3][dw < 4 ? 0 : 1], big);
-        };
-        auto prep_table = [&](int j) {
-            const int key = (dw & 3) * 32 + lane;
-            const uint32_t at = (base + j) & 3;
-            // 2^-e puts the largest into [2^10, 2^12)
-            const int e = max((int)(emax[at][dw < 4 ? 0 : 1] >> 7) - 127 - 10, -100);
+            for (int i = 0; i < 4; ++i) big = max(big, max(w[i] & 0x7fffu, (w[i] >> 16) & 0x7fffu));
+#pragma unroll
+            for (int o = 1; o < LPR; o <<= 1) big = max(big, __shfl_xor_sync(0xffffffffu, big, o));
+            const int e = max((int)(big >> 7) - 127, -100) - 10;
             const float f = pow2i(max(-e, -126));
-            uint32_t* t = tab + (((base + j) & 1) * 2 + (dw < 4 ? 0 : 1)) * (G * kKeys) + key;
+            float v[8];
 #pragma unroll
-            for (int i = 0; i < G; ++i)
-                t[i * kKeys] = f16x2_of(__uint_as_float(pr[i] << 16) * f, __uint_as_float(pr[i] & 0xffff0000u) * f);
-            if ((dw & 3) == 0 && lane == 0) expo[at][dw < 4 ? 0 : 1] = dw < 4 ? pow2i(min(e, 127)) : (float)e;
-        };
-        if (warp > kWarpMma && n > 0) {
-            fetch_page(0);
-            unit_at(0);
-            load_pr();
-            load_k();
-            load_v();
-            if (n > 1) fetch_page(1);
-        }
-
-        // queries: D / 8 lanes per row, scaled by a power of two to a maximum in [2^10, 2^11)
-        if (warp != kWarpMma) {
-            constexpr int LPR = D / 8, RPW = 32 / LPR;
-            const int wi = warp < kWarpMma ? warp : warp - 1;
-            for (int r0 = wi * RPW; r0 < kRows; r0 += (kSoft + kDeq) * RPW) {
-                const int r = r0 + lane / LPR, c = lane % LPR;
-                uint4 x = make_uint4(0u, 0u, 0u, 0u);
-                if (r < nrows) {
-                    const int rr = it.row0 + r;
-                    x = *reinterpret_cast<const uint4*>(a.q + (int64_t)(s.q0 + rr / a.group) * a.q_ts +
-                                                        (int64_t)(h * a.group + rr % a.group) * a.q_hs + c * 8);
-                }
-                const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-                uint32_t big = 0;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) big = max(big, max(w[i] & 0x7fffu, (w[i] >> 16) & 0x7fffu));
-#pragma unroll
-                for (int o = 1; o < LPR; o <<= 1) big = max(big, __shfl_xor_sync(0xffffffffu, big, o));
-                const int e = max((int)(big >> 7) - 127, -100) - 10;
-                const float f = pow2i(max(-e, -126));
-                float v[8];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    v[2 * i] = __uint_as_float(w[i] << 16) * f;
-                    v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u) * f;
-                }
-                uint4 y;
-                if (BITS == 4)
-                    y = make_uint4(f16x2_of(v[0], v[4]), f16x2_of(v[1], v[5]), f16x2_of(v[2], v[6]), f16x2_of(v[3], v[7]));
-                else
-                    y = make_uint4(f16x2_of(v[0], v[1]), f16x2_of(v[2], v[3]), f16x2_of(v[4], v[5]), f16x2_of(v[6], v[7]));
-                *reinterpret_cast<uint4*>(sq + (c >> 3) * (kRows * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = y;
-                if (c == 0) qsr[r] = a.scale_log2 * pow2i(min(e, 127));
+            for (int i = 0; i < 4; ++i) {
+                v[2 * i] = __uint_as_float(w[i] << 16) * f;
+                v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u) * f;
             }
-            fence_proxy_async_smem();
+            uint4 y;
+            if (BITS == 4)
+                y = make_uint4(f16x2_of(v[0], v[4]), f16x2_of(v[1], v[5]), f16x2_of(v[2], v[6]), f16x2_of(v[3], v[7]));
+            else
+                y = make_uint4(f16x2_of(v[0], v[1]), f16x2_of(v[2], v[3]), f16x2_of(v[4], v[5]), f16x2_of(v[6], v[7]));
+            *reinterpret_cast<uint4*>(sq + (c >> 3) * (kRows * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = y;
+            if (c == 0) qsr[r] = a.scale_log2 * pow2i(min(e, 127));
         }
-        __syncthreads();
+        fence_proxy_async_smem();
+    };
+    uint32_t base = 0;  // steps of the CTA's earlier items (barrier phases run on)
 
-        if (warp == kWarpMma) {
-            if (lane == 0 && n > 0) {
+    if (warp < kWarpDeq) {
+        regs_up<C::REGS_SOFT>();
+        for (;;) {
+            if (tid == 0) item_s = *abort ? total : atomicAdd(&work.head[0], 1);
+            sync_all();
+            const int id = item_s;
+            if (id >= total) break;
+            const Item it = work.items[id / a.pool.kv_heads];
+            const int h = id % a.pool.kv_heads, n = it.k1 - it.k0;
+            const SeqSpan s = seq_span(a, it.b);
+            const int nrows = min(kRows, s.n * a.group - it.row0);
+            load_queries(it, s, h, nrows);
+            sync_all();
+            const int quarter = warp & 3, half = warp >> 2;
+            const uint32_t lane_base = (uint32_t)(32 * quarter) << 16;
+            const int r = quarter * 32 + lane, rr = it.row0 + r;
+            const float sr = qsr[r];
+            const int lim = r < nrows ? min(s.len, s.len - s.n + rr / a.group + 1) : 0;
+            const int low = min(s.len, s.len - s.n + (it.row0 + quarter * 32) / a.group + 1);  // the warp's first row sees least
+            const bool short_tile = quarter * 32 + 32 > nrows;
+            const uint32_t oc = tmem_o + lane_base + half * (D / 2);  // this thread's columns of O
+            float m = -INFINITY, l = 0.f;
+            bool ok = true;
+            for (int j = 0; j < n; ++j) {
+                const uint32_t gj = base + j;
+                const int pos = (it.k0 + j) * kKeys + half * 64;
+                // on an abort the pair still meets at its barrier, once a step
+                ok = ok && warp_wait<true>(&efull[gj & 3], (gj / 4) & 1, abort) && warp_wait<true>(&sfull[gj % SB], (gj / SB) & 1, abort);
+                if (!ok) {
+                    pair_barrier(quarter);
+                    continue;
+                }
+                tc_fence_after();
+                const float4* ex = expo + (gj & 3) * 8 + half * 4;
+                const uint32_t ts = tmem + lane_base + (gj % SB) * kKeys + half * 64;
+                const bool mask = pos + 64 > low || short_tile;
+                // scores of columns 32 q .. 32 q + 31, -inf where the row does not see the position
+                uint32_t x[C::KEEP ? 64 : 32];
+                auto fetch = [&](int q, uint32_t (&v)[32]) {
+                    tmem_ld32(ts + q * 32, v);
+                    tmem_wait_ld();
+                    if (mask) {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if (pos + q * 32 + i >= lim) v[i] = 0xff800000u;
+                    }
+                };
+                float xm = -INFINITY;
+                if constexpr (C::KEEP) {
+                    tmem_ld32(ts, reinterpret_cast<uint32_t(&)[32]>(x[0]));
+                    tmem_ld32(ts + 32, reinterpret_cast<uint32_t(&)[32]>(x[32]));
+                    tmem_wait_ld();
+                    if (mask) {
+#pragma unroll
+                        for (int i = 0; i < 64; ++i)
+                            if (pos + i >= lim) x[i] = 0xff800000u;
+                    }
+                }
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    if constexpr (!C::KEEP) fetch(q, reinterpret_cast<uint32_t(&)[32]>(x));
+#pragma unroll
+                    for (int y = 0; y < 2; ++y) {
+                        const uint32_t* z = x + (C::KEEP ? q * 32 : 0) + y * 16;
+                        float m0 = __uint_as_float(z[0]), m1 = __uint_as_float(z[1]);
+#pragma unroll
+                        for (int i = 2; i < 16; i += 4) {
+                            m0 = fmaxf(fmaxf(m0, __uint_as_float(z[i])), __uint_as_float(z[i + 1]));
+                            if (i + 2 < 16) m1 = fmaxf(fmaxf(m1, __uint_as_float(z[i + 2])), __uint_as_float(z[i + 3]));
+                        }
+                        m0 = fmaxf(m0, m1);
+                        const float4 e = ex[q * 2 + y];
+                        if (m0 > -INFINITY) xm = fmaxf(xm, fmaf(m0, sr * e.x, e.y));
+                    }
+                }
+                float* xc = xch + (gj & 1) * (2 * kRows);
+                xc[half * kRows + r] = xm;
+                pair_barrier(quarter);
+                xm = fmaxf(xm, xc[(half ^ 1) * kRows + r]);
+                const bool grow = xm > m + kLazy || (m == -INFINITY && xm > -INFINITY);
+                if (__any_sync(0xffffffffu, grow)) {
+                    const float by = grow ? ex2(m - xm) : 1.f;  // 0 from -inf
+                    if (j > 0) {
+                        ok = warp_wait<true>(&pdone[(gj - 1) % SB], ((gj - 1) / SB) & 1, abort);
+                        tc_fence_after();
+#pragma unroll 1
+                        for (int q = 0; q < D / 32; ++q) {
+                            uint32_t z[16];
+                            tmem_ld16(oc + q * 16, z);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) z[i] = __float_as_uint(__uint_as_float(z[i]) * by);
+                            tmem_st16(oc + q * 16, z);
+                        }
+                    }
+                    l *= by;
+                    if (grow) m = xm;
+                }
+                const float mm = m == -INFINITY ? 0.f : m;
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    if constexpr (!C::KEEP) fetch(q, reinterpret_cast<uint32_t(&)[32]>(x));
+                    uint32_t p[16];
+#pragma unroll
+                    for (int y = 0; y < 2; ++y) {
+                        const uint32_t* z = x + (C::KEEP ? q * 32 : 0) + y * 16;
+                        const float4 e = ex[q * 2 + y];
+                        const uint64_t c = f32x2(sr * e.x, sr * e.x), off = f32x2(e.y - mm, e.y - mm);
+                        uint64_t sum = 0;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            float p0, p1;
+                            f32x2_split(f32x2_fma(f32x2(__uint_as_float(z[2 * i]), __uint_as_float(z[2 * i + 1])), c, off), p0, p1);
+                            p0 = ex2(p0);
+                            p1 = ex2(p1);
+                            sum = f32x2_add(sum, f32x2(p0, p1));
+                            p[8 * y + i] = f16x2_of(p0, p1);
+                        }
+                        float s0, s1;
+                        f32x2_split(sum, s0, s1);
+                        l = fmaf(s0 + s1, e.z, l);
+                    }
+                    tmem_st16(ts + q * 16, p);
+                }
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&pfull[gj % SB]);
+            }
+            // output: half of this thread's row
+            if (n > 0 && ok) ok = warp_wait<true>(&pdone[(base + n - 1) % SB], ((base + n - 1) / SB) & 1, abort);
+            tc_fence_after();
+            float* xc = xch + ((base + n) & 1) * (2 * kRows);
+            xc[half * kRows + r] = l;
+            pair_barrier(quarter);
+            if (ok) {
+                l += xc[(half ^ 1) * kRows + r];
+                const bool whole = it.slot < 0;
+                const int slot = it.slot * a.pool.kv_heads + h;
+                const float inv = l == 0.f ? 0.f : 1.f / l;
+                uint16_t* y = a.out + ((int64_t)(s.q0 + rr / a.group) * a.heads + h * a.group + rr % a.group) * D + half * (D / 2);
+                float* po = work.o + ((int64_t)slot * kRows + r) * D + half * (D / 2);
+                if (!whole && r < nrows && half == 0) work.ml[(int64_t)slot * kRows + r] = make_float2(m, l);
+#pragma unroll 1
+                for (int q = 0; q < D / 64; ++q) {
+                    uint32_t x[32];
+                    if (n > 0) {
+                        tmem_ld32(oc + q * 32, x);
+                        tmem_wait_ld();
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) x[i] = 0u;
+                    }
+                    if (r < nrows) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            float v[8];
+#pragma unroll
+                            for (int i = 0; i < 8; ++i)  // back to the features' own order
+                                v[i] = __uint_as_float(x[8 * e + (BITS == 4 ? (i & 3) * 2 + (i >> 2) : i)]);
+                            if (whole) {
+                                *reinterpret_cast<uint4*>(y + q * 32 + e * 8) =
+                                    make_uint4(bf16x2_of(v[0] * inv, v[1] * inv), bf16x2_of(v[2] * inv, v[3] * inv),
+                                               bf16x2_of(v[4] * inv, v[5] * inv), bf16x2_of(v[6] * inv, v[7] * inv));
+                            } else {
+                                float4* z = reinterpret_cast<float4*>(po + q * 32 + e * 8);
+                                z[0] = make_float4(v[0], v[1], v[2], v[3]);
+                                z[1] = make_float4(v[4], v[5], v[6], v[7]);
+                            }
+                        }
+                    }
+                    __syncwarp();
+                }
+            }
+            tc_fence_before();
+            base += n;
+            sync_all();  // queries, TMEM and the item's number are free for the next item
+            tc_fence_after();
+        }
+    } else if (warp < kWarpMma) {
+        regs_up<C::REGS_DEQ>();
+        for (;;) {
+            sync_all();
+            const int id = item_s;
+            if (id >= total) break;
+            const Item it = work.items[id / a.pool.kv_heads];
+            const int h = id % a.pool.kv_heads, n = it.k1 - it.k0;
+            const SeqSpan s = seq_span(a, it.b);
+            const int nrows = min(kRows, s.n * a.group - it.row0);
+
+            // dequantizing warps: the codes of the first step on their way before anything else
+            const int dw = warp - kWarpDeq, pu = a.pool.page_units;
+            uint4 kr[UPW][KC], vr[C::ONE ? 1 : UPW][KC];
+            uint32_t pr[UPW][G];
+            const uint8_t* ua[UPW];          // the units of the step whose keys are loaded last
+            const uint8_t* uv[UPW];          // those of the step whose values are loaded next
+            int pi[UPW], ri[UPW], pg[UPW];   // page and unit in the page one step further, and its table entry
+            int last_page = 0;
+            auto fetch_pages = [&]() {       // entries behind the last position repeat the last page (masked later)
+#pragma unroll
+                for (int u = 0; u < UPW; ++u) pg[u] = a.table[(int64_t)it.b * a.table_stride + min(pi[u], last_page)];
+            };
+            auto next_units = [&]() {        // looks at the entries only now: their load is a step old
+#pragma unroll
+                for (int u = 0; u < UPW; ++u) {
+                    if (pg[u] < 0 || pg[u] >= a.pool.pages) {
+                        record_device_error(kDevErrBadIndex);
+                        pg[u] = 0;
+                    }
+                    ua[u] = a.pool.data + (((int64_t)pg[u] * a.pool.kv_heads + h) * pu + ri[u]) * (int64_t)C::UB;
+                    pi[u] += 8 / pu;
+                    ri[u] += 8 % pu;
+                    if (ri[u] >= pu) {
+                        ri[u] -= pu;
+                        ++pi[u];
+                    }
+                }
+            };
+            auto load_pr = [&]() {  // lanes 0-15: the keys' rows, 16-31: the values'
+#pragma unroll
+                for (int u = 0; u < UPW; ++u) {
+                    const uint8_t* p = ua[u] + (lane < 16 ? kv_key_pair(lane, 0, C::RB, G) : kv_value_pair(lane - 16, 0, C::RB, G));
+                    if constexpr (G == 4) {
+                        const uint4 x = __ldg(reinterpret_cast<const uint4*>(p));
+                        pr[u][0] = x.x, pr[u][1] = x.y, pr[u][2] = x.z, pr[u][3] = x.w;
+                    } else if constexpr (G == 2) {
+                        const uint2 x = __ldg(reinterpret_cast<const uint2*>(p));
+                        pr[u][0] = x.x, pr[u][1] = x.y;
+                    } else {
+                        pr[u][0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+                    }
+                }
+            };
+            // A warp's 512 bytes: keys 8 rows of one 64-byte panel (or all 16 of a 32-byte row), values two
+            // pieces of all 16 rows; eight neighbouring lanes hold eight rows (no bank conflict when they store).
+            const int krow = C::RB >= 64 ? lane & 7 : (lane & 7) + 8 * (lane >> 4);
+            const int vrow = (lane & 3) * 2 + ((lane >> 2) & 1) + 8 * (lane >> 4);
+            auto load_k = [&]() {
+#pragma unroll
+                for (int u = 0; u < UPW; ++u)
+#pragma unroll
+                    for (int i = 0; i < KC; ++i)
+                        kr[u][i] = __ldg(reinterpret_cast<const uint4*>(
+                            ua[u] + (C::RB >= 64 ? (i >> 1) * 1024 + (i & 1) * 512 + krow * 64 + (lane >> 3) * 16 : krow * 32 + ((lane >> 3) & 1) * 16)));
+            };
+            auto load_v = [&](uint4 (&r)[UPW][KC]) {
+#pragma unroll
+                for (int u = 0; u < UPW; ++u)
+#pragma unroll
+                    for (int i = 0; i < KC; ++i)
+                        r[u][i] = __ldg(reinterpret_cast<const uint4*>(uv[u] + kKvRows * (C::RB + 4 * G) + i * 512 + (lane >> 4) * 256 +
+                                                                       ((lane >> 2) & 1) * 128 + ((lane >> 3) & 1) * 64 + (lane & 3) * 16));
+            };
+            if (n > 0) {
+                last_page = ((s.len + kKvRows - 1) / kKvRows - 1) / pu;
+#pragma unroll
+                for (int u = 0; u < UPW; ++u) {
+                    const int unit = it.k0 * 8 + dw * UPW + u;
+                    pi[u] = unit / pu;
+                    ri[u] = unit % pu;
+                }
+                fetch_pages();
+                next_units();
+                if (n > 1) fetch_pages();
+                load_pr();
+                load_k();
+#pragma unroll
+                for (int u = 0; u < UPW; ++u) uv[u] = ua[u];
+                if constexpr (!C::ONE) load_v(vr);
+            }
+            load_queries(it, s, h, nrows);
+            sync_all();
+            // Keys run one step ahead of values: K of step j + 1 while P V of step j - 1 runs, V of step j while
+            // Q K^T of step j + 1 does, so that one buffer of each (dim 256) keeps the tensor pipe fed.
+            bool ok = true;  // warp-uniform
+            auto keys = [&](int j) {
+                const uint32_t gj = base + j, st = gj % NB, use = gj / NB;
+                // exponents and f16 (scale, bias) of this warp's units, of keys and values
+#pragma unroll
+                for (int u = 0; u < UPW; ++u) {
+                    const int unit = dw * UPW + u, row = lane & 15, isv = lane >> 4;
+                    uint32_t big = 0;
+#pragma unroll
+                    for (int i = 0; i < G; ++i) {
+                        if ((it.k0 + j) * kKeys + unit * kKvRows + row >= s.len) pr[u][i] = 0u;  // behind the last position: zeros
+                        const uint32_t sc = pr[u][i] & 0x7fffu, bi = (pr[u][i] >> 16) & 0x7fffu;
+                        // |value| <= max(|bias|, 16 or 256 |scale|) up to a factor of two
+                        big = max(big, max(bi, sc ? sc + (BITS << 7) : 0u));
+                    }
+                    // 2^-e puts the largest into [2^10, 2^12)
+                    const int ek = max((int)(__reduce_max_sync(0xffffffffu, isv ? 0u : big) >> 7) - 137, -100);
+                    const int ev = max((int)(__reduce_max_sync(0xffffffffu, isv ? big : 0u) >> 7) - 137, -100);
+                    const float f = pow2i(max(isv ? -ev : -ek, -126));
+                    uint32_t* t = tab + (((gj & 1) * 8 + unit) * 2 + isv) * (G * 16) + row;
+#pragma unroll
+                    for (int i = 0; i < G; ++i)
+                        t[i * 16] = f16x2_of(__uint_as_float(pr[u][i] << 16) * f, __uint_as_float(pr[u][i] & 0xffff0000u) * f);
+                    if (lane == 0) expo[(gj & 3) * 8 + unit] = make_float4(pow2i(min(ek, 127)), (float)ev, pow2i(max(-ev, -126)), 0.f);
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&efull[gj & 3]);
+                ok = ok && (use == 0 || warp_wait<true>(&kfree[st], (use - 1) & 1, abort));
+                if (ok) {
+                    uint8_t* kb = sk + st * C::KB;
+#pragma unroll
+                    for (int u = 0; u < UPW; ++u)
+#pragma unroll
+                        for (int i = 0; i < KC; ++i) {
+                            const int unit = dw * UPW + u, row = C::RB >= 64 ? (i & 1) * 8 + krow : krow;
+                            const int dim = (C::RB >= 64 ? (i >> 1) * 64 + (lane >> 3) * 16 : ((lane >> 3) & 1) * 16) * 8 / BITS;
+                            dequant_piece<BITS>(kr[u][i], tab[(((gj & 1) * 8 + unit) * 2 * G + (dim >> 6)) * 16 + row],
+                                                kb + (dim >> 6) * (kKeys * 128) + (unit * 16 + row) * 128, (dim & 63) >> 3, row & 7);
+                        }
+                    fence_proxy_async_smem();
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&kfull[st]);
+            };
+            auto load_keys = [&](int j) {  // of step j, and the table entries of the one after
+                next_units();
+                if (j + 1 < n) fetch_pages();
+                load_pr();
+                load_k();
+            };
+            if (n > 0) keys(0);
+            if (n > 1) load_keys(1);
+            for (int j = 0; j < n && ok; ++j) {
+                const uint32_t gj = base + j, st = gj % NB, use = gj / NB;
+                if (j + 1 < n) keys(j + 1);
+                if constexpr (C::ONE) {
+                    load_v(kr);
+                } else {
+#pragma unroll
+                    for (int u = 0; u < UPW; ++u) uv[u] = ua[u];
+                    if (j + 2 < n) load_keys(j + 2);
+                }
+                ok = ok && (use == 0 || warp_wait<true>(&vfree[st], (use - 1) & 1, abort));
+                if (ok) {
+                    uint8_t* vb = sv + st * C::KB;
+#pragma unroll
+                    for (int u = 0; u < UPW; ++u)
+#pragma unroll
+                        for (int i = 0; i < KC; ++i) {
+                            const int unit = dw * UPW + u, dim = (i * 2 + ((lane >> 3) & 1)) * 128 / BITS;
+                            const uint4& x = C::ONE ? kr[u][i] : vr[C::ONE ? 0 : u][i];
+                            dequant_piece<BITS>(x, tab[((((gj & 1) * 8 + unit) * 2 + 1) * G + (dim >> 6)) * 16 + vrow],
+                                                vb + (dim >> 6) * (kKeys * 128) + (unit * 16 + vrow) * 128, (dim & 63) >> 3, vrow & 7);
+                        }
+                    fence_proxy_async_smem();
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&vfull[st]);
+                if constexpr (C::ONE) {
+#pragma unroll
+                    for (int u = 0; u < UPW; ++u) uv[u] = ua[u];
+                    if (j + 2 < n) load_keys(j + 2);
+                } else {
+                    if (j + 1 < n) load_v(vr);
+                }
+            }
+            base += n;
+            sync_all();
+        }
+    } else {
+        regs_down<C::REGS_MMA>();
+        for (;;) {
+            sync_all();
+            const int id = item_s;
+            if (id >= total) break;
+            const Item it = work.items[id / a.pool.kv_heads];
+            const int n = it.k1 - it.k0;
+            sync_all();
+            tc_fence_after();
+            if (warp == kWarpMma && lane == 0 && n > 0) {
                 const uint32_t idesc_s = umma_idesc_f16(kRows, kKeys), idesc_o = umma_idesc_f16(kRows, D) | kIdescBMn;
                 const uint64_t qd = umma_desc_sw128(sq), kd0 = umma_desc_sw128(sk), vd0 = umma_desc_mn_sw128(sv, kKeys * 128);
                 auto qk = [&](int j) {
@@ -469,11 +780,13 @@ __global__ void __launch_bounds__(kThreads, 1) attn_chunk_kernel(const __grid_co
                     if (gj >= SB && !thread_wait<true>(&pdone[gj % SB], (gj / SB - 1) & 1, abort)) return false;
                     tc_fence_after();
                     const uint64_t kd = kd0 + (uint64_t)((st * C::KB) >> 4);
+#pragma unroll 1  // short loops: unrolled, the issuer waits for its instructions (16 products 3100 cycles)
+                    for (int p = 0; p < D / 64; ++p)
 #pragma unroll
-                    for (int k = 0; k < D / 16; ++k) {
-                        const uint64_t off = (uint64_t)(((k >> 2) * (kRows * 128) + (k & 3) * 32) >> 4);
-                        umma_smem_a(tmem + (gj % SB) * kKeys, qd + off, kd + off, idesc_s, k > 0);
-                    }
+                        for (int k = 0; k < 4; ++k) {
+                            const uint64_t off = (uint64_t)(p * (kRows * 128 >> 4) + k * 2);
+                            umma_smem_a(tmem + (gj % SB) * kKeys, qd + off, kd + off, idesc_s, p > 0 || k > 0);
+                        }
                     umma_commit(&kfree[st]);
                     umma_commit(&sfull[gj % SB]);
                     return true;
@@ -486,201 +799,20 @@ __global__ void __launch_bounds__(kThreads, 1) attn_chunk_kernel(const __grid_co
                     if (!ok) break;
                     tc_fence_after();
                     const uint64_t vd = vd0 + (uint64_t)((st * C::KB) >> 4);
+#pragma unroll 1
+                    for (int p = 0; p < 2; ++p)  // P: 64 positions in 32 columns at the start of each half of S
 #pragma unroll
-                    for (int k = 0; k < kKeys / 16; ++k)
-                        umma_tmem_a(tmem_o, tmem + (gj % SB) * kKeys + k * 8, vd + (uint64_t)((k * 16 * 128) >> 4), idesc_o, j > 0 || k > 0);
+                        for (int k = 0; k < 4; ++k)
+                            umma_tmem_a(tmem_o, tmem + (gj % SB) * kKeys + p * 64 + k * 8, vd + (uint64_t)((p * 4 + k) * (16 * 128 >> 4)),
+                                        idesc_o, j > 0 || p > 0 || k > 0);
                     umma_commit(&vfree[st]);
                     umma_commit(&pdone[gj % SB]);
                 }
             }
-        } else if (warp > kWarpMma) {
-            bool ok = true;
-            if (n > 0) {
-                prep_max(0);
-                deq_barrier();
-                prep_table(0);
-                if (tid == 5 * 32) emax[(base + 1) & 3][0] = emax[(base + 1) & 3][1] = 0u;
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&efull[base & 3]);
-                deq_barrier();
-            }
-            for (int j = 0; j < n; ++j) {
-                const uint32_t gj = base + j, st = gj % NB, use = gj / NB;
-                const uint32_t* t = tab + (gj & 1) * (2 * G * kKeys);
-                const bool more = j + 1 < n;
-                // ok stays warp-uniform; on an abort the warps still meet at every barrier
-                ok = ok && (use == 0 || warp_wait<true>(&kfree[st], (use - 1) & 1, abort));
-                uint8_t* kb = sk + st * C::KB;
-                if (ok) {
-#pragma unroll
-                    for (int i = 0; i < KC; ++i) {
-                        const int blk = dw + 8 * i;
-                        int key, dim;  // dim: first feature of the piece
-                        if (C::RB >= 64) {
-                            key = (blk & 15) * 8 + (lane & 7);
-                            dim = ((blk >> 4) * 64 + (lane >> 3) * 16) * 8 / BITS;
-                        } else {
-                            key = blk * 16 + (lane & 7) + 8 * (lane >> 4);
-                            dim = ((lane >> 3) & 1) * 32;
-                        }
-                        dequant_piece<BITS>(kr[i], t[(dim >> 6) * kKeys + key], kb + (dim >> 6) * (kKeys * 128) + key * 128, (dim & 63) >> 3, key & 7);
-                    }
-                    fence_proxy_async_smem();
-                }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&kfull[st]);
-                if (more) {
-                    unit_at(j + 1);
-                    load_pr();
-                    load_k();
-                    if (j + 2 < n) fetch_page(j + 2);
-                }
-                ok = ok && (use == 0 || warp_wait<true>(&vfree[st], (use - 1) & 1, abort));
-                uint8_t* vb = sv + st * C::KB;
-                if (ok) {
-#pragma unroll
-                    for (int i = 0; i < KC; ++i) {
-                        const int blk = dw + 8 * i, c = (blk >> 3) * 2 + ((lane >> 3) & 1);
-                        const int key = (blk & 7) * 16 + (lane & 3) * 2 + ((lane >> 2) & 1) + 8 * (lane >> 4);
-                        const int dim = c * 128 / BITS;
-                        dequant_piece<BITS>(vr[i], t[(G + (dim >> 6)) * kKeys + key], vb + (dim >> 6) * (kKeys * 128) + key * 128, (dim & 63) >> 3, key & 7);
-                    }
-                    fence_proxy_async_smem();
-                }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&vfull[st]);
-                if (more) {
-                    load_v();
-                    prep_max(j + 1);
-                    deq_barrier();
-                    prep_table(j + 1);
-                    if (tid == 5 * 32) emax[(gj + 2) & 3][0] = emax[(gj + 2) & 3][1] = 0u;
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&efull[(gj + 1) & 3]);
-                    deq_barrier();
-                }
-            }
-        } else {
-            const uint32_t lane_base = (uint32_t)(32 * warp) << 16;
-            const int r = warp * 32 + lane, rr = it.row0 + r;
-            const float sr = qsr[r];
-            const int lim = r < nrows ? min(s.len, s.len - s.n + rr / a.group + 1) : 0;
-            const int low = min(s.len, s.len - s.n + (it.row0 + warp * 32) / a.group + 1);  // the warp's first row sees least
-            float m = -INFINITY, l = 0.f;
-            bool ok = true;
-            for (int j = 0; j < n; ++j) {
-                const uint32_t gj = base + j;
-                const int pos = (it.k0 + j) * kKeys;
-                ok = warp_wait<true>(&efull[gj & 3], (gj / 4) & 1, abort) && warp_wait<true>(&sfull[gj % SB], (gj / SB) & 1, abort);
-                if (!ok) break;
-                tc_fence_after();
-                const float c = sr * expo[gj & 3][0], ev = expo[gj & 3][1];
-                const uint32_t ts = tmem + lane_base + (gj % SB) * kKeys;
-                const bool mask = pos + kKeys > low || r >= nrows;
-                float mx = -INFINITY;
-                uint32_t x[32];
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    tmem_ld32(ts + q * 32, x);
-                    tmem_wait_ld();
-                    if (__any_sync(0xffffffffu, mask)) {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) mx = fmaxf(mx, pos + q * 32 + i < lim ? __uint_as_float(x[i]) : -INFINITY);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) mx = fmaxf(mx, __uint_as_float(x[i]));
-                    }
-                }
-                const float xm = mx == -INFINITY ? -INFINITY : fmaf(mx, c, ev);
-                const bool grow = xm > m + kLazy || (m == -INFINITY && xm > -INFINITY);
-                if (__any_sync(0xffffffffu, grow)) {
-                    const float by = grow ? ex2(m - xm) : 1.f;  // 0 from -inf
-                    if (j > 0) {
-                        if (!(ok = warp_wait<true>(&pdone[(gj - 1) % SB], ((gj - 1) / SB) & 1, abort))) break;
-                        tc_fence_after();
-#pragma unroll 1
-                        for (int q = 0; q < D / 32; ++q) {
-                            tmem_ld32(tmem_o + lane_base + q * 32, x);
-                            tmem_wait_ld();
-#pragma unroll
-                            for (int i = 0; i < 32; ++i) x[i] = __float_as_uint(__uint_as_float(x[i]) * by);
-                            tmem_st32(tmem_o + lane_base + q * 32, x);
-                        }
-                    }
-                    l *= by;
-                    if (grow) m = xm;
-                }
-                const float off = m == -INFINITY ? 0.f : ev - m;
-                float sum = 0.f;
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    tmem_ld32(ts + q * 32, x);
-                    tmem_wait_ld();
-                    uint32_t p[16];
-                    if (__any_sync(0xffffffffu, mask)) {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if (pos + q * 32 + i >= lim) x[i] = 0xff800000u;  // -inf
-                    }
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const float p0 = ex2(fmaf(__uint_as_float(x[2 * i]), c, off)), p1 = ex2(fmaf(__uint_as_float(x[2 * i + 1]), c, off));
-                        sum += p0 + p1;
-                        p[i] = f16x2_of(p0, p1);
-                    }
-                    tmem_st16(ts + q * 16, p);
-                }
-                l = fmaf(sum, ex2(-ev), l);
-                tmem_wait_st();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&pfull[gj % SB]);
-            }
-            // output: this thread's row
-            if (n > 0 && ok) ok = warp_wait<true>(&pdone[(base + n - 1) % SB], ((base + n - 1) / SB) & 1, abort);
-            tc_fence_after();
-            if (ok) {
-                const bool whole = it.slot < 0;
-                const int slot = it.slot * a.pool.kv_heads + h;
-                const float inv = l == 0.f ? 0.f : 1.f / l;
-                uint16_t* y = a.out + ((int64_t)(s.q0 + rr / a.group) * a.heads + h * a.group + rr % a.group) * D;
-                float* po = work.o + ((int64_t)slot * kRows + r) * D;
-                if (!whole && r < nrows) work.ml[(int64_t)slot * kRows + r] = make_float2(m, l);
-#pragma unroll 1
-                for (int q = 0; q < D / 32; ++q) {
-                    uint32_t x[32];
-                    if (n > 0) {
-                        tmem_ld32(tmem_o + lane_base + q * 32, x);
-                        tmem_wait_ld();
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) x[i] = 0u;
-                    }
-                    if (r < nrows)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        float v[8];
-#pragma unroll
-                        for (int i = 0; i < 8; ++i)  // back to the features' own order
-                            v[i] = __uint_as_float(x[8 * e + (BITS == 4 ? (i & 3) * 2 + (i >> 2) : i)]);
-                        if (whole) {
-                            *reinterpret_cast<uint4*>(y + q * 32 + e * 8) =
-                                make_uint4(bf16x2_of(v[0] * inv, v[1] * inv), bf16x2_of(v[2] * inv, v[3] * inv),
-                                           bf16x2_of(v[4] * inv, v[5] * inv), bf16x2_of(v[6] * inv, v[7] * inv));
-                        } else {
-                            float4* z = reinterpret_cast<float4*>(po + q * 32 + e * 8);
-                            z[0] = make_float4(v[0], v[1], v[2], v[3]);
-                            z[1] = make_float4(v[4], v[5], v[6], v[7]);
-                        }
-                    }
-                    __syncwarp();
-                }
-            }
-            tc_fence_before();
+            __syncwarp();
+            base += n;
+            sync_all();
         }
-        base += n;
-        __syncthreads();  // queries, TMEM and the item's number are free for the next item
-        tc_fence_after();
     }
     if (warp == kWarpMma) {
         if (lane == 0) {
@@ -753,12 +885,18 @@ cudaError_t run_chunk(const AttnArgs& a, cudaStream_t stream) {
     using C = ChunkCfg<D, BITS>;
     cudaError_t e = cudaFuncSetAttribute(attn_chunk_kernel<D, BITS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM);
     if (e != cudaSuccess) return e;
+    // the warpgroups' register shares have to fit what the block is launched with, or their increase waits for good
+    static const int regs = [] {
+        cudaFuncAttributes f{};
+        return cudaFuncGetAttributes(&f, attn_chunk_kernel<D, BITS>) == cudaSuccess ? f.numRegs : 0;
+    }();
+    if (regs * C::THREADS < C::REGS_ALL) return cudaErrorInvalidConfiguration;
     const int sms = device_num_sms();
     const int64_t tiles = tiles_most(a.tokens, a.group, a.batch);
     const ChunkWork w = chunk_work(a.part, tiles, sms, a.pool.kv_heads);
     e = launch_chunk(attn_plan_kernel, dim3(1), 1024, 0, a.pdl, stream, a, w, tiles, sms);
     if (e != cudaSuccess) return e;
-    e = launch_chunk(attn_chunk_kernel<D, BITS>, dim3(sms), kThreads, C::SMEM, a.pdl, stream, a, w);
+    e = launch_chunk(attn_chunk_kernel<D, BITS>, dim3(sms), C::THREADS, C::SMEM, a.pdl, stream, a, w);
     if (e != cudaSuccess) return e;
     const int64_t cuts = std::min(tiles, slots_most(sms, a.pool.kv_heads) / 2);
     return launch_chunk(attn_chunk_join_kernel<D>, dim3((unsigned)cuts, a.pool.kv_heads, kRows / 16), 256, 0, a.pdl, stream, a, w);
