@@ -19,7 +19,8 @@
 // memory); 8 dequantize, each its own unit of a step, codes prefetched to registers straight from the pages;
 // one issues the MMAs; two go ahead, look the pages up and turn scales, biases and exponents of a step into
 // shared-memory tables.  Two tiles per CTA on the same keys (256 rows, dim 128) were measured and left out:
-// with one S buffer a tile the weights wait for both products and a step of both took 7000 cycles.
+// with one S buffer a tile the weights wait for both products and a step of both took 7000 cycles.  So was a
+// row per thread with two groups of softmax warps taking turns at the steps: 251 us where this takes 205.
 // Work: a planning kernel lays the tiles' steps (plus kItemCost each) of all heads end to end and cuts them
 // into equal shares, one per CTA, from the lengths on the device; a tile cut between CTAs is joined from
 // binary32 partial rows in a fixed order.
@@ -222,10 +223,11 @@ struct ChunkCfg {
     static constexpr uint32_t TAB = 8 * 2 * G * 16 * 4;   // f16 (scale, bias) of a step: [unit][K, V][group][row]
     static constexpr uint32_t OFF_E = OFF_T + kRing * TAB;      // exponents [ring][unit]: 2^eK, e, 2^-e
     static constexpr uint32_t OFF_A = OFF_E + kRing * 8 * 16;   // where a step's units stand [ring][unit]
-    static constexpr uint32_t OFF_X = OFF_A + kRing * 8 * 8;    // [2 steps][column half][row]: maxima (dim 256)
-    static constexpr uint32_t OFF_SR = OFF_X + 2 * 2 * kRows * 4;
-    static constexpr uint32_t OFF_BAR = OFF_SR + kRows * 4;
+    static constexpr uint32_t OFF_X = OFF_A + kRing * 8 * 8;    // [2 steps in turn, end][column half][row]: maxima, sums
+    static constexpr uint32_t OFF_SR = OFF_X + 3 * 2 * kRows * 4;
+    static constexpr uint32_t OFF_BAR = OFF_SR + 2 * kRows * 4;
     static constexpr uint32_t SMEM = 1024 + OFF_BAR + 256;
+    static_assert(NB * KB >= kSoft * 4096);  // rows are turned there on their way out
 };
 
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
@@ -255,6 +257,11 @@ __device__ __forceinline__ uint64_t umma_desc_mn_sw128(const void* smem_ptr, uin
 }
 constexpr uint32_t kIdescBMn = 1u << 16;  // B is MN-major
 
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p;
+}
 // the two warps of a TMEM lane quarter
 __device__ __forceinline__ void pair_barrier(int quarter) { asm volatile("bar.sync %0, 64;" ::"r"(quarter + 1) : "memory"); }
 
@@ -443,7 +450,9 @@ __global__ void __launch_bounds__(ChunkCfg<D, BITS>::THREADS, 1)
     uint64_t* pdone = pfull + SB;      // [SB] MMA commit: P V done
     uint64_t* efull = pdone + SB;      // [kRing] table warps
     uint64_t* efree = efull + kRing;   // [kRing] softmax and dequantizing warps
-    uint64_t* fin = efree + kRing;     // [1]
+    uint64_t* qready = efree + kRing;  // [2 items in turn] dequantizing warps: queries and their factors are in place
+    uint64_t* odone = qready + 2;      // [1] softmax warps: an item's rows have left
+    uint64_t* fin = odone + 1;         // [1] the last MMAs
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_s;
     volatile int* abort = &abort_s;
@@ -470,6 +479,9 @@ __global__ void __launch_bounds__(ChunkCfg<D, BITS>::THREADS, 1)
             mbar_init(&efull[i], 2);
             mbar_init(&efree[i], kSoft + DW);
         }
+        mbar_init(&qready[0], DW);
+        mbar_init(&qready[1], DW);
+        mbar_init(odone, kSoft);
         mbar_init(fin, 1);
         fence_mbar_init();
     }
@@ -481,47 +493,10 @@ __global__ void __launch_bounds__(ChunkCfg<D, BITS>::THREADS, 1)
     pdl_launch_dependents();
     const int item0 = work.first[blockIdx.x], item1 = work.first[blockIdx.x + 1];
 
-    // Every warp meets the others twice an item: the last one done, queries in place.
-    auto sync_all = [] { asm volatile("bar.sync 0, %0;" ::"n"(C::THREADS) : "memory"); };
-    // Queries, by the softmax and dequantizing warps: D / 8 lanes per row, scaled by a power of two to a
-    // maximum in [2^10, 2^11)
-    auto load_queries = [&](const Item& it, const SeqSpan& s, int nrows) {
-        constexpr int LPR = D / 8, RPW = 32 / LPR;
-        const int rows = (nrows + kRows - 1) / kRows * kRows;
-        for (int r0 = warp * RPW; r0 < rows; r0 += (kSoft + DW) * RPW) {
-            const int r = r0 + lane / LPR, c = lane % LPR;
-            uint4 x = make_uint4(0u, 0u, 0u, 0u);
-            if (r < nrows) {
-                const int rr = it.row0 + r;
-                x = *reinterpret_cast<const uint4*>(a.q + (int64_t)(s.q0 + rr / a.group) * a.q_ts +
-                                                    (int64_t)(it.h * a.group + rr % a.group) * a.q_hs + c * 8);
-            }
-            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-            uint32_t big = 0;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) big = max(big, max(w[i] & 0x7fffu, (w[i] >> 16) & 0x7fffu));
-#pragma unroll
-            for (int o = 1; o < LPR; o <<= 1) big = max(big, __shfl_xor_sync(0xffffffffu, big, o));
-            const int e = max((int)(big >> 7) - 127, -100) - 10;
-            const float f = pow2i(max(-e, -126));
-            float v[8];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                v[2 * i] = __uint_as_float(w[i] << 16) * f;
-                v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u) * f;
-            }
-            uint4 y;
-            if (BITS == 4)
-                y = make_uint4(f16x2_of(v[0], v[4]), f16x2_of(v[1], v[5]), f16x2_of(v[2], v[6]), f16x2_of(v[3], v[7]));
-            else
-                y = make_uint4(f16x2_of(v[0], v[1]), f16x2_of(v[2], v[3]), f16x2_of(v[4], v[5]), f16x2_of(v[6], v[7]));
-            *reinterpret_cast<uint4*>(sq + (r / kRows) * (kRows * D * 2) + (c >> 3) * (kRows * 128) + (r % kRows) * 128 +
-                                      (((c & 7) ^ (r & 7)) << 4)) = y;
-            if (c == 0) qsr[r] = a.scale_log2 * pow2i(min(e, 127));
-        }
-        fence_proxy_async_smem();
-    };
+    // Roles meet only at the barriers of what they hand on: the dequantizing and table warps run into the next
+    // item while this one's rows leave.
     uint32_t base = 0;  // steps of the CTA's earlier items (barrier phases run on)
+    uint32_t busy = 0;  // its earlier items that have steps
 
     if (warp < kWarpDeq) {
         set_registers<C::REGS_LAUNCH, C::REGS_SOFT>();
@@ -533,17 +508,13 @@ __global__ void __launch_bounds__(ChunkCfg<D, BITS>::THREADS, 1)
             const Item it = work.items[i];
             const int n = it.k1 - it.k0;
             const SeqSpan s = seq_span(a, it.b);
-            const int nrows = min(kRows, s.n * a.group - it.row0);
-            load_queries(it, s, nrows);
-            sync_all();
-            tc_fence_after();
-            const int rr = it.row0 + r;
-            const float sr = qsr[r];
+            const int nrows = min(kRows, s.n * a.group - it.row0), rr = it.row0 + r;
+            bool ok = n == 0 || warp_wait<true>(&qready[busy & 1], (busy >> 1) & 1, abort);
+            const float sr = qsr[(busy & 1) * kRows + r];
             const int lim = r < nrows ? min(s.len, s.len - s.n + rr / a.group + 1) : 0;
             const int low = min(s.len, s.len - s.n + (it.row0 + quarter * 32) / a.group + 1);  // the warp's first row sees least
             const bool short_tile = quarter * 32 + 32 > nrows;
             float m = -INFINITY, l = 0.f;
-            bool ok = true;
             for (int j = 0; j < n; ++j) {
                 const uint32_t gj = base + j, sl = gj % kRing;
                 ok = ok && warp_wait<true>(&efull[sl], (gj / kRing) & 1, abort) && warp_wait<true>(&sfull[gj % SB], (gj / SB) & 1, abort);
@@ -584,52 +555,70 @@ __global__ void __launch_bounds__(ChunkCfg<D, BITS>::THREADS, 1)
                 }
             }
             // output: half of the columns of this thread's row
-            if (n > 0 && ok) ok = warp_wait<true>(&pdone[(base + n - 1) % SB], ((base + n - 1) / SB) & 1, abort);
-            float* xc = xch + ((base + n) & 1) * (2 * kRows);
-            xc[upper * kRows + r] = l;
-            pair_barrier(quarter);
-            l += xc[(upper ^ 1) * kRows + r];
+            if (n > 0) {
+                ok = ok && warp_wait<true>(&pdone[(base + n - 1) % SB], ((base + n - 1) / SB) & 1, abort);
+                float* xc = xch + 2 * (2 * kRows);
+                xc[upper * kRows + r] = l;
+                pair_barrier(quarter);
+                l += xc[(upper ^ 1) * kRows + r];
+            }
             tc_fence_after();
-            if (ok) {
+            if (n == 0) {  // none of the rows sees a position
+                for (int c = 0; c < D / 2 && r < nrows; c += 8)
+                    *reinterpret_cast<uint4*>(a.out + ((int64_t)(s.q0 + rr / a.group) * a.heads + it.h * a.group + rr % a.group) * D +
+                                              upper * (D / 2) + c) = make_uint4(0u, 0u, 0u, 0u);
+            } else if (ok) {
                 const bool whole = it.slot < 0;
                 const float inv = l == 0.f ? 0.f : 1.f / l;
-                uint16_t* y = a.out + ((int64_t)(s.q0 + rr / a.group) * a.heads + it.h * a.group + rr % a.group) * D + upper * (D / 2);
-                float* po = work.o + ((int64_t)it.slot * kRows + r) * D + upper * (D / 2);
                 if (!whole && r < nrows && upper == 0) work.ml[(int64_t)it.slot * kRows + r] = make_float2(m, l);
+                // 32 rows x 32 columns at a time through the values' memory (every product is done), so that a
+                // row's columns leave side by side
+                uint8_t* stage = sv + warp * 4096;
+                const int64_t at = whole ? ((int64_t)(s.q0 + rr / a.group) * a.heads + it.h * a.group + rr % a.group) * D
+                                         : ((int64_t)it.slot * kRows + r) * D;
 #pragma unroll 1
                 for (int q = 0; q < D / 64; ++q) {
+                    const int c0 = upper * (D / 2) + q * 32;
                     uint32_t x[32];
-                    if (n > 0) {
-                        tmem_ld32(oc + q * 32, x);
-                        tmem_wait_ld();
+                    tmem_ld32(tmem_o + lane_base + c0, x);
+                    tmem_wait_ld();
+                    auto col = [&](int c) { return __uint_as_float(x[(c & ~7) + (BITS == 4 ? (c & 3) * 2 + ((c >> 2) & 1) : (c & 7))]); };
+                    if (whole) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            *reinterpret_cast<uint4*>(stage + (lane * 4 + (e ^ ((lane >> 1) & 3))) * 16) =
+                                make_uint4(bf16x2_of(col(8 * e) * inv, col(8 * e + 1) * inv), bf16x2_of(col(8 * e + 2) * inv, col(8 * e + 3) * inv),
+                                           bf16x2_of(col(8 * e + 4) * inv, col(8 * e + 5) * inv), bf16x2_of(col(8 * e + 6) * inv, col(8 * e + 7) * inv));
                     } else {
 #pragma unroll
-                        for (int c = 0; c < 32; ++c) x[c] = 0u;
+                        for (int e = 0; e < 8; ++e)
+                            *reinterpret_cast<float4*>(stage + (lane * 8 + (e ^ (lane & 7))) * 16) =
+                                make_float4(col(4 * e), col(4 * e + 1), col(4 * e + 2), col(4 * e + 3));
                     }
-                    if (r < nrows) {
+                    __syncwarp();
+                    if (whole) {
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            float v[8];
+                            const int row = e * 8 + (lane >> 2), f = lane & 3;
+                            const int64_t to = __shfl_sync(0xffffffffu, at, row);
+                            const uint4 v = lds128(stage + (row * 4 + (f ^ ((row >> 1) & 3))) * 16);
+                            if (quarter * 32 + row < nrows) *reinterpret_cast<uint4*>(a.out + to + c0 + f * 8) = v;
+                        }
+                    } else {
 #pragma unroll
-                            for (int c = 0; c < 8; ++c)  // back to the features' own order
-                                v[c] = __uint_as_float(x[8 * e + (BITS == 4 ? (c & 3) * 2 + (c >> 2) : c)]);
-                            if (whole) {
-                                *reinterpret_cast<uint4*>(y + q * 32 + e * 8) =
-                                    make_uint4(bf16x2_of(v[0] * inv, v[1] * inv), bf16x2_of(v[2] * inv, v[3] * inv),
-                                               bf16x2_of(v[4] * inv, v[5] * inv), bf16x2_of(v[6] * inv, v[7] * inv));
-                            } else {
-                                float4* z = reinterpret_cast<float4*>(po + q * 32 + e * 8);
-                                z[0] = make_float4(v[0], v[1], v[2], v[3]);
-                                z[1] = make_float4(v[4], v[5], v[6], v[7]);
-                            }
+                        for (int e = 0; e < 8; ++e) {
+                            const int row = e * 4 + (lane >> 3), f = lane & 7;
+                            const int64_t to = __shfl_sync(0xffffffffu, at, row);
+                            const uint4 v = lds128(stage + (row * 8 + (f ^ (row & 7))) * 16);
+                            if (quarter * 32 + row < nrows) *reinterpret_cast<uint4*>(work.o + to + c0 + f * 4) = v;
                         }
                     }
                     __syncwarp();
                 }
             }
-            tc_fence_before();
+            if (lane == 0 && n > 0) mbar_arrive(odone);
+            busy += n > 0;
             base += n;
-            sync_all();  // queries and TMEM are free for the next item
         }
     } else if (warp < kWarpMma) {
         set_registers<C::REGS_LAUNCH, C::REGS_DEQ>();
@@ -641,12 +630,64 @@ __global__ void __launch_bounds__(ChunkCfg<D, BITS>::THREADS, 1)
         const int vrow = (lane & 3) * 2 + ((lane >> 2) & 1) + 8 * (lane >> 4);
         const uint32_t kat = C::RB >= 64 ? krow * 64 + (lane >> 3) * 16 : krow * 32 + ((lane >> 3) & 1) * 16;
         const uint32_t vat = kKvRows * (C::RB + 4 * G) + (lane >> 4) * 256 + ((lane >> 2) & 1) * 128 + ((lane >> 3) & 1) * 64 + (lane & 3) * 16;
+        bool ok = true;  // warp-uniform
         for (int i = item0; i < item1; ++i) {
             const Item it = work.items[i];
             const int n = it.k1 - it.k0;
-            const SeqSpan s = seq_span(a, it.b);
-            const int nrows = min(kRows, s.n * a.group - it.row0);
-            bool ok = true;  // warp-uniform
+            if (n == 0) continue;
+            // Queries: LPR lanes per row, each row scaled by a power of two to a maximum in [2^10, 2^11).  They go
+            // in once the last item's scores are done, while its weights, products and rows are still under way.
+            {
+                constexpr int LPR = D / 8, RPW = 32 / LPR, STEP = DW * RPW, BATCH = D == 256 ? 8 : kRows / STEP;
+                const SeqSpan s = seq_span(a, it.b);
+                const int nrows = min(kRows, s.n * a.group - it.row0), c = lane % LPR;
+                int row = dw * RPW + lane / LPR, g = (it.row0 + row) % a.group;
+                const int dt = STEP / a.group, dg = STEP - dt * a.group;
+                const uint16_t* qp = a.q + (int64_t)(s.q0 + (it.row0 + row) / a.group) * a.q_ts + (int64_t)(it.h * a.group + g) * a.q_hs + c * 8;
+                const int64_t dq = dt * a.q_ts + dg * a.q_hs, wrap = a.q_ts - a.group * a.q_hs;
+#pragma unroll 1
+                for (int r0 = 0; r0 < kRows / (STEP * BATCH); ++r0) {
+                    uint4 q[BATCH];
+#pragma unroll
+                    for (int k = 0; k < BATCH; ++k) {
+                        q[k] = row + k * STEP < nrows ? *reinterpret_cast<const uint4*>(qp) : make_uint4(0u, 0u, 0u, 0u);
+                        qp += dq;
+                        g += dg;
+                        if (g >= a.group) {
+                            g -= a.group;
+                            qp += wrap;
+                        }
+                    }
+                    if (r0 == 0 && base > 0) ok = ok && warp_wait<true>(&kfree[(base - 1) % NB], ((base - 1) / NB) & 1, abort);
+#pragma unroll
+                    for (int k = 0; k < BATCH; ++k, row += STEP) {
+                        const uint32_t w[4] = {q[k].x, q[k].y, q[k].z, q[k].w};
+                        uint32_t big = __vmaxu2(__vmaxu2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu), __vmaxu2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
+                        big = max(big & 0xffffu, big >> 16);
+                        if constexpr (LPR == 32) {
+                            big = __reduce_max_sync(0xffffffffu, big);
+                        } else {
+#pragma unroll
+                            for (int o = 1; o < LPR; o <<= 1) big = max(big, __shfl_xor_sync(0xffffffffu, big, o));
+                        }
+                        const int e = max((int)(big >> 7) - 127, -100) - 10;
+                        const float f = pow2i(max(-e, -126));
+                        float v[8];
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) {
+                            v[2 * x] = __uint_as_float(w[x] << 16) * f;
+                            v[2 * x + 1] = __uint_as_float(w[x] & 0xffff0000u) * f;
+                        }
+                        *reinterpret_cast<uint4*>(sq + (c >> 3) * (kRows * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4)) =
+                            BITS == 4 ? make_uint4(f16x2_of(v[0], v[4]), f16x2_of(v[1], v[5]), f16x2_of(v[2], v[6]), f16x2_of(v[3], v[7]))
+                                      : make_uint4(f16x2_of(v[0], v[1]), f16x2_of(v[2], v[3]), f16x2_of(v[4], v[5]), f16x2_of(v[6], v[7]));
+                        if (c == 0) qsr[(busy & 1) * kRows + row] = a.scale_log2 * pow2i(min(e, 127));
+                    }
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&qready[busy & 1]);
+            }
             auto load_keys = [&](int j) {
                 const uint32_t gj = base + j;
                 ok = ok && warp_wait<true>(&efull[gj % kRing], (gj / kRing) & 1, abort);
@@ -679,17 +720,13 @@ __global__ void __launch_bounds__(ChunkCfg<D, BITS>::THREADS, 1)
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&kfull[st]);
             };
-            if (n > 0) {
-                load_keys(0);
-                if constexpr (!C::ONE) {
-                    if (ok) load_values(0, vr);
-                }
+            load_keys(0);
+            if constexpr (!C::ONE) {
+                if (ok) load_values(0, vr);
             }
-            load_queries(it, s, nrows);
-            sync_all();
             // Keys run one step ahead of values: K of step j + 1 while P V of step j - 1 runs, V of step j while
             // Q K^T of step j + 1 does, so that one buffer of each (dim 256) keeps the tensor pipe fed.
-            if (n > 0) keys(0);
+            keys(0);
             if (n > 1) load_keys(1);
             for (int j = 0; j < n; ++j) {
                 const uint32_t gj = base + j, st = gj % NB, use = gj / NB;
@@ -699,6 +736,7 @@ __global__ void __launch_bounds__(ChunkCfg<D, BITS>::THREADS, 1)
                 } else {
                     if (j + 2 < n) load_keys(j + 2);
                 }
+                if (j == 0) ok = ok && (busy == 0 || warp_wait<true>(odone, (busy - 1) & 1, abort));
                 ok = ok && (use == 0 || warp_wait<true>(&vfree[st], (use - 1) & 1, abort));
                 if (ok) {
                     uint8_t* vb = sv + st * C::KB;
@@ -722,8 +760,8 @@ __global__ void __launch_bounds__(ChunkCfg<D, BITS>::THREADS, 1)
                     if (j + 1 < n && ok) load_values(j + 1, vr);
                 }
             }
+            ++busy;
             base += n;
-            sync_all();
         }
     } else {
         set_registers<C::REGS_LAUNCH, C::REGS_MMA>();
@@ -732,50 +770,55 @@ __global__ void __launch_bounds__(ChunkCfg<D, BITS>::THREADS, 1)
             const Item it = work.items[i];
             const int n = it.k1 - it.k0;
             if (tw < 0) {
-                sync_all();
-                tc_fence_after();
-                if (lane == 0 && n > 0) {
+                if (n > 0 && warp_wait<true>(&qready[busy & 1], (busy >> 1) & 1, abort)) {
+                    tc_fence_after();
                     const uint32_t idesc_s = umma_idesc_f16(kRows, kKeys), idesc_o = umma_idesc_f16(kRows, D) | kIdescBMn;
                     const uint64_t qd0 = umma_desc_sw128(sq), kd0 = umma_desc_sw128(sk), vd0 = umma_desc_mn_sw128(sv, kKeys * 128);
                     auto qk = [&](int j) {
                         const uint32_t gj = base + j, st = gj % NB;
-                        if (!thread_wait<true>(&kfull[st], (gj / NB) & 1, abort)) return false;
+                        if (!warp_wait<true>(&kfull[st], (gj / NB) & 1, abort)) return false;
                         // S of step j goes where P of step j - SB stands: that product has to be done
-                        if (gj >= SB && !thread_wait<true>(&pdone[gj % SB], (gj / SB - 1) & 1, abort)) return false;
+                        if (gj >= SB && !warp_wait<true>(&pdone[gj % SB], (gj / SB - 1) & 1, abort)) return false;
                         tc_fence_after();
                         const uint64_t kd = kd0 + (uint64_t)((st * C::KB) >> 4);
                         const uint32_t d = tmem + (gj % SB) * kKeys;
+                        if (elect_one()) {
 #pragma unroll 1  // short loops: unrolled, the issuer waits for its instructions (16 products 3100 cycles)
-                        for (int p = 0; p < D / 64; ++p)
+                            for (int p = 0; p < D / 64; ++p)
 #pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                const uint64_t off = (uint64_t)(p * (kRows * 128 >> 4) + k * 2);
-                                umma_smem_a(d, qd0 + off, kd + off, idesc_s, p > 0 || k > 0);
-                            }
-                        umma_commit(&kfree[st]);
-                        umma_commit(&sfull[gj % SB]);
+                                for (int k = 0; k < 4; ++k) {
+                                    const uint64_t off = (uint64_t)(p * (kRows * 128 >> 4) + k * 2);
+                                    umma_smem_a(d, qd0 + off, kd + off, idesc_s, p > 0 || k > 0);
+                                }
+                            umma_commit(&kfree[st]);
+                            umma_commit(&sfull[gj % SB]);
+                        }
+                        __syncwarp();
                         return true;
                     };
                     bool ok = qk(0);
                     for (int j = 0; j < n && ok; ++j) {
                         if (j + 1 < n && !(ok = qk(j + 1))) break;
                         const uint32_t gj = base + j, st = gj % NB;
-                        ok = thread_wait<true>(&vfull[st], (gj / NB) & 1, abort) && thread_wait<true>(&pfull[gj % SB], (gj / SB) & 1, abort);
+                        ok = warp_wait<true>(&vfull[st], (gj / NB) & 1, abort) && warp_wait<true>(&pfull[gj % SB], (gj / SB) & 1, abort);
                         if (!ok) break;
                         tc_fence_after();
                         const uint64_t vd = vd0 + (uint64_t)((st * C::KB) >> 4);
                         const uint32_t pw = tmem + (gj % SB) * kKeys;  // 64 positions in 32 columns, at the start of each half of S
+                        if (elect_one()) {
 #pragma unroll 1
-                        for (int p = 0; p < 2; ++p)
+                            for (int p = 0; p < 2; ++p)
 #pragma unroll
-                            for (int k = 0; k < 4; ++k)
-                                umma_tmem_a(tmem_o, pw + p * 64 + k * 8, vd + (uint64_t)((p * 4 + k) * (16 * 128 >> 4)), idesc_o,
-                                            j > 0 || p > 0 || k > 0);
-                        umma_commit(&vfree[st]);
-                        umma_commit(&pdone[gj % SB]);
+                                for (int k = 0; k < 4; ++k)
+                                    umma_tmem_a(tmem_o, pw + p * 64 + k * 8, vd + (uint64_t)((p * 4 + k) * (16 * 128 >> 4)), idesc_o,
+                                                j > 0 || p > 0 || k > 0);
+                            umma_commit(&vfree[st]);
+                            umma_commit(&pdone[gj % SB]);
+                        }
+                        __syncwarp();
                     }
                 }
-                __syncwarp();
+                busy += n > 0;
             } else if (tw < 2) {
                 // Tables of units 4 tw .. 4 tw + 3: lanes 0-15 hold the keys' rows of a unit, 16-31 the values'.
                 const SeqSpan s = seq_span(a, it.b);
@@ -856,14 +899,9 @@ __global__ void __launch_bounds__(ChunkCfg<D, BITS>::THREADS, 1)
                         load_pairs_of();
                         if (j + 2 < n) fetch_page();
                     }
-                    if (j == 0) sync_all();  // the dequantizing warps load their first codes before they meet
                 }
-                if (n == 0) sync_all();
-            } else {
-                sync_all();
             }
             base += n;
-            sync_all();
         }
     }
     if (warp == kWarpMma) {
