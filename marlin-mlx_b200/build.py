@@ -1,9 +1,10 @@
-"""Build the product library libmarlin_q4.so in-tree (nvcc, sm_100a only).
+"""Build the product library libmarlin_q4.so (nvcc, sm_100a only) and the compiled torch front end
+_attention.so (g++, torch's headers and libraries) in-tree.
 
     python marlin-mlx_b200/build.py            # incremental
     python marlin-mlx_b200/build.py --force    # rebuild everything
 
-Objects go to marlin-mlx_b200/_build/, the shared library to marlin-mlx_b200/marlin_q4/.
+Objects go to marlin-mlx_b200/_build/, the shared libraries to marlin-mlx_b200/marlin_q4/.
 """
 from __future__ import annotations
 
@@ -19,6 +20,8 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 BUILD = PKG / "_build"
 LIB = PKG / "marlin_q4" / "libmarlin_q4.so"
+FRONT_SRC = CSRC / "attention_torch.cpp"
+FRONT = PKG / "marlin_q4" / "_attention.so"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr",
@@ -38,6 +41,29 @@ def sources() -> list[Path]:
 
 def headers() -> list[Path]:
     return sorted(list(CSRC.glob("*.cuh")) + list(CSRC.glob("*.h")) + list((ROOT / "include").glob("*.h")))
+
+
+def build_front(force: bool = False, verbose: bool = False) -> Path:
+    import importlib.util
+    import sysconfig
+
+    newest = max(FRONT_SRC.stat().st_mtime, (ROOT / "include" / "marlin_q4.h").stat().st_mtime)
+    torch = Path(importlib.util.find_spec("torch").origin).parent
+    newest = max(newest, (torch / "version.py").stat().st_mtime)
+    if not force and FRONT.exists() and FRONT.stat().st_mtime >= newest:
+        return FRONT
+    cuda = Path(nvcc()).resolve().parent.parent
+    include = [ROOT / "include", torch / "include", torch / "include" / "torch" / "csrc" / "api" / "include", cuda / "include",
+               sysconfig.get_paths()["include"]]
+    # the shared libstdc++ by name: torch's exceptions and streams cross into this module, and some compilers
+    # link theirs in statically
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", *(f"-I{i}" for i in include),
+           str(FRONT_SRC), "-o", str(FRONT), f"-L{torch / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda",
+           "-l:libstdc++.so.6"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    subprocess.run(cmd, check=True)
+    return FRONT
 
 
 def build(force: bool = False, verbose: bool = False, ptxas_info: bool = False) -> Path:
@@ -60,6 +86,7 @@ def build(force: bool = False, verbose: bool = False, ptxas_info: bool = False) 
         if verbose:
             print(" ".join(cmd), flush=True)
         subprocess.run(cmd, check=True)
+    build_front(force, verbose)
     return LIB
 
 

@@ -1,0 +1,247 @@
+// attention_torch.cpp — torch front end of the attention operators: argument checks, outputs and the call.
+//
+// A decode step calls these operators on a few rows, where the kernels take 2 to 5 us: the host's share of a
+// call is what counts.  Checked in Python and called through ctypes, qk_norm_rope took 15 us of host time,
+// kv_write 7 and paged_attention 14, of which the launch is 3; here they take 6, 3.1 and 5.4.  The library stays
+// the one that the package has loaded: bind() is given its entry points.
+#include <Python.h>
+
+#include <ATen/core/Tensor.h>
+#include <ATen/ops/empty.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/python_variable.h>
+
+#include <cmath>
+#include <initializer_list>
+
+#include "marlin_q4.h"
+
+namespace {
+
+struct Library {
+    decltype(&marlin_q4_kv_unit_bytes) unit_bytes;
+    decltype(&marlin_q4_qk_norm_rope) qk_norm_rope;
+    decltype(&marlin_q4_kv_write) kv_write;
+    decltype(&marlin_q4_kv_read) kv_read;
+    decltype(&marlin_q4_paged_attention_workspace_size) workspace_size;
+    decltype(&marlin_q4_paged_attention) paged_attention;
+} lib{};
+
+const at::Tensor& tensor(PyObject* o, const char* name) {
+    TORCH_CHECK_TYPE(THPVariable_Check(o), name, " must be a tensor");
+    return THPVariable_Unpack(o);
+}
+int64_t integer(PyObject* o) {
+    const long long v = PyLong_AsLongLong(o);
+    if (v == -1 && PyErr_Occurred()) throw python_error();
+    return v;
+}
+double real(PyObject* o) {
+    const double v = PyFloat_AsDouble(o);
+    if (v == -1.0 && PyErr_Occurred()) throw python_error();
+    return v;
+}
+
+int32_t code(at::ScalarType t, const char* name) {
+    TORCH_CHECK_TYPE(t == at::kBFloat16 || t == at::kFloat, name, " must be bfloat16 or float32, got ", t);
+    return t == at::kBFloat16 ? MARLIN_Q4_BF16 : MARLIN_Q4_F32;
+}
+// A [tokens, heads, head_dim] operand
+int32_t heads(const at::Tensor& t, const char* name) {
+    TORCH_CHECK_VALUE(t.dim() == 3, name, " must be [tokens, heads, head_dim], got ", t.sizes());
+    const int32_t c = code(t.scalar_type(), name);
+    TORCH_CHECK_VALUE(t.stride(2) == 1, name, "'s features must be contiguous");
+    return c;
+}
+void int32s(const at::Tensor& t, const char* name, std::initializer_list<int64_t> shape) {
+    TORCH_CHECK_TYPE(t.scalar_type() == at::kInt, name, " must be int32, got ", t.scalar_type());
+    TORCH_CHECK_VALUE(t.sizes() == at::IntArrayRef(shape) && t.is_contiguous(), name, " must be contiguous ", at::IntArrayRef(shape),
+                      ", got ", t.sizes());
+}
+// All of them on one CUDA device, which is returned
+c10::DeviceIndex device(const at::Tensor& first, std::initializer_list<const at::Tensor*> others) {
+    TORCH_CHECK_VALUE(first.is_cuda(), "expected CUDA tensors");
+    for (const at::Tensor* t : others)
+        TORCH_CHECK_VALUE(!t || t->device() == first.device(), "tensors on different devices: ", first.device(), " and ", t->device());
+    return first.get_device();
+}
+marlin_q4_kv_cache pool(const at::Tensor& data, PyObject* head_dim, PyObject* bits) {
+    const int64_t dim = integer(head_dim), b = integer(bits);
+    const int64_t unit = dim > 0 && dim <= 256 && b > 0 && b <= 8 ? (int64_t)lib.unit_bytes((int32_t)dim, (int32_t)b) : 0;
+    TORCH_CHECK_VALUE(unit != 0, "unsupported head_dim ", dim, " or bits ", b, " (64, 128, 256; 4, 8)");
+    TORCH_CHECK_VALUE(data.scalar_type() == at::kByte && data.dim() == 4 && data.size(3) == unit && data.is_contiguous(),
+                      "data must be contiguous uint8 [pages, kv_heads, page_size / 16, ", unit, "]");
+    TORCH_CHECK_VALUE(data.size(1) <= INT32_MAX && data.size(2) <= INT32_MAX / 16, "unsupported cache ", data.sizes());
+    marlin_q4_kv_cache c{};
+    c.data = data.data_ptr();
+    c.pages = data.size(0);
+    c.page_size = (int32_t)(data.size(2) * 16);
+    c.kv_heads = (int32_t)data.size(1);
+    c.head_dim = (int32_t)dim;
+    c.bits = (int32_t)b;
+    return c;
+}
+at::Tensor fresh(at::IntArrayRef shape, at::ScalarType type, const at::Tensor& like) {
+    return at::empty(shape, like.options().dtype(type));
+}
+bool given(PyObject* o) { return o != Py_None; }
+PyObject* two(at::Tensor a, at::Tensor b) {
+    PyObject* r = PyTuple_New(2);
+    if (!r) throw python_error();
+    PyTuple_SET_ITEM(r, 0, THPVariable_Wrap(std::move(a)));
+    PyTuple_SET_ITEM(r, 1, THPVariable_Wrap(std::move(b)));
+    return r;
+}
+void arguments(Py_ssize_t got, Py_ssize_t want) {
+    TORCH_CHECK_TYPE(got == want, "expected ", want, " arguments, got ", got);
+    TORCH_CHECK(lib.paged_attention, "the library has not been bound");
+}
+
+// Each returns what the caller gets, or the library's status where that is not 0.
+
+PyObject* qk_norm_rope(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    arguments(n, 10);
+    const at::Tensor &q = tensor(a[0], "q"), &k = tensor(a[1], "k"), &qw = tensor(a[2], "q_weight"), &kw = tensor(a[3], "k_weight"),
+                     &positions = tensor(a[4], "positions"), &freqs = tensor(a[5], "inv_freq");
+    const int32_t type = heads(q, "q");
+    heads(k, "k");
+    const bool half = a[9] == Py_True;  // bf16 outputs
+    TORCH_CHECK_TYPE(q.scalar_type() == k.scalar_type(), "q and k must have one dtype");
+    const int64_t t = q.size(0), h = q.size(1), d = q.size(2), kvh = k.size(1);
+    TORCH_CHECK_VALUE(k.size(0) == t && k.size(2) == d, "k ", k.sizes(), " does not match q ", q.sizes());
+    TORCH_CHECK_VALUE(positions.dim() == 1 || positions.dim() == 2, "positions must be [tokens] or [axes, tokens], got ", positions.sizes());
+    const int64_t axes = positions.dim() == 1 ? 1 : positions.size(0);
+    if (positions.dim() == 1)
+        int32s(positions, "positions", {t});
+    else
+        int32s(positions, "positions", {axes, t});
+    for (const at::Tensor* w : {&qw, &kw})
+        TORCH_CHECK_VALUE(w->scalar_type() == at::kBFloat16 && w->dim() == 1 && w->size(0) == d && w->is_contiguous(),
+                          w == &qw ? "q_weight" : "k_weight", " must be contiguous bfloat16 [", d, "]");
+    TORCH_CHECK_VALUE(freqs.scalar_type() == at::kFloat && freqs.dim() == 1 && freqs.is_contiguous(),
+                      "inv_freq must be contiguous float32 [rot_dim / 2]");
+    const uint8_t* axis_of = nullptr;
+    if (given(a[7])) {
+        TORCH_CHECK_VALUE(PyBytes_Check(a[7]) && PyBytes_GET_SIZE(a[7]) == freqs.numel(), "axes must name one axis per pair");
+        axis_of = reinterpret_cast<const uint8_t*>(PyBytes_AS_STRING(a[7]));
+    }
+    const int adjacent = PyObject_IsTrue(a[6]);
+    if (adjacent < 0) throw python_error();
+    const double eps = real(a[8]);
+    TORCH_CHECK_VALUE(h <= INT32_MAX && kvh <= INT32_MAX && d <= INT32_MAX && axes <= INT32_MAX && freqs.numel() <= INT32_MAX / 2,
+                      "unsupported sizes");
+    const c10::DeviceIndex dev = device(q, {&k, &qw, &kw, &positions, &freqs});
+    const c10::cuda::CUDAGuard guard(dev);
+    const at::ScalarType to = half ? at::kBFloat16 : at::kFloat;
+    at::Tensor qo = fresh({t, h, d}, to, q), ko = fresh({t, kvh, d}, to, q);
+    const int status = lib.qk_norm_rope(q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1), type, t, (int32_t)h,
+                                        (int32_t)kvh, (int32_t)d, static_cast<const uint16_t*>(qw.data_ptr()), static_cast<const uint16_t*>(kw.data_ptr()), (float)eps,
+                                        static_cast<const int32_t*>(positions.data_ptr()), (int32_t)axes, axis_of,
+                                        static_cast<const float*>(freqs.data_ptr()), (int32_t)(2 * freqs.numel()), adjacent, qo.data_ptr(),
+                                        ko.data_ptr(), half ? MARLIN_Q4_BF16 : MARLIN_Q4_F32, c10::cuda::getCurrentCUDAStream(dev).stream());
+    return status ? PyLong_FromLong(status) : two(std::move(qo), std::move(ko));
+    END_HANDLE_TH_ERRORS
+}
+
+PyObject* kv_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    arguments(n, 6);
+    const at::Tensor &data = tensor(a[0], "data"), &k = tensor(a[3], "k"), &v = tensor(a[4], "v"), &slots = tensor(a[5], "slots");
+    const marlin_q4_kv_cache c = pool(data, a[1], a[2]);
+    const int32_t type = heads(k, "k");
+    heads(v, "v");
+    TORCH_CHECK_VALUE(k.size(1) == c.kv_heads && k.size(2) == c.head_dim && k.sizes() == v.sizes() && k.scalar_type() == v.scalar_type(),
+                      "k ", k.sizes(), " and v ", v.sizes(), " must be [tokens, ", c.kv_heads, ", ", c.head_dim, "] of one dtype");
+    int32s(slots, "slots", {k.size(0)});
+    const c10::DeviceIndex dev = device(data, {&k, &v, &slots});
+    const c10::cuda::CUDAGuard guard(dev);
+    const int status = lib.kv_write(&c, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0), v.stride(1), type,
+                                    static_cast<const int32_t*>(slots.data_ptr()), k.size(0), c10::cuda::getCurrentCUDAStream(dev).stream());
+    return PyLong_FromLong(status);
+    END_HANDLE_TH_ERRORS
+}
+
+PyObject* kv_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    arguments(n, 4);
+    const at::Tensor &data = tensor(a[0], "data"), &slots = tensor(a[3], "slots");
+    const marlin_q4_kv_cache c = pool(data, a[1], a[2]);
+    const int64_t t = slots.numel();
+    int32s(slots, "slots", {t});
+    const c10::DeviceIndex dev = device(data, {&slots});
+    const c10::cuda::CUDAGuard guard(dev);
+    at::Tensor k = fresh({t, c.kv_heads, c.head_dim}, at::kBFloat16, data), v = fresh({t, c.kv_heads, c.head_dim}, at::kBFloat16, data);
+    const int status = lib.kv_read(&c, static_cast<const int32_t*>(slots.data_ptr()), t, static_cast<uint16_t*>(k.data_ptr()),
+                                   static_cast<uint16_t*>(v.data_ptr()), c10::cuda::getCurrentCUDAStream(dev).stream());
+    return status ? PyLong_FromLong(status) : two(std::move(k), std::move(v));
+    END_HANDLE_TH_ERRORS
+}
+
+PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    arguments(n, 11);
+    const at::Tensor &q = tensor(a[0], "q"), &data = tensor(a[1], "data"), &table = tensor(a[4], "block_table"), &lens = tensor(a[5], "kv_lens");
+    const at::Tensor* cu = given(a[6]) ? &tensor(a[6], "cu_q") : nullptr;
+    const at::Tensor* out = given(a[9]) ? &tensor(a[9], "out") : nullptr;
+    const at::Tensor* work = given(a[10]) ? &tensor(a[10], "workspace") : nullptr;
+    const marlin_q4_kv_cache c = pool(data, a[2], a[3]);
+    TORCH_CHECK_VALUE(q.dim() == 3, "q must be [tokens, heads, head_dim], got ", q.sizes());
+    TORCH_CHECK_TYPE(q.scalar_type() == at::kBFloat16, "q must be bfloat16, got ", q.scalar_type());
+    TORCH_CHECK_VALUE(q.stride(2) == 1, "q's features must be contiguous");
+    const int64_t t = q.size(0), h = q.size(1), d = q.size(2);
+    TORCH_CHECK_VALUE(d == c.head_dim, "q's head_dim ", d, " is not the cache's ", c.head_dim);
+    TORCH_CHECK_VALUE(table.scalar_type() == at::kInt && table.dim() == 2, "block_table must be int32 [batch, pages]");
+    const int64_t batch = table.size(0), width = table.size(1);
+    TORCH_CHECK_VALUE(width <= 1 || table.stride(1) == 1, "block_table's rows must be contiguous");
+    int32s(lens, "kv_lens", {batch});
+    if (cu) int32s(*cu, "cu_q", {batch + 1});
+    const int64_t max_q = integer(a[7]);
+    const float scale = given(a[8]) ? (float)real(a[8]) : (float)std::pow((double)d, -0.5);
+    if (out)
+        TORCH_CHECK_VALUE(out->scalar_type() == at::kBFloat16 && out->sizes() == q.sizes() && out->is_contiguous(),
+                          "out must be contiguous bfloat16 ", q.sizes());
+    if (work) TORCH_CHECK_VALUE(work->scalar_type() == at::kByte && work->is_contiguous(), "workspace must be contiguous uint8");
+    TORCH_CHECK_VALUE(h <= INT32_MAX && batch < INT32_MAX && width <= INT32_MAX && max_q >= INT32_MIN && max_q <= INT32_MAX,
+                      "unsupported sizes");
+    const c10::DeviceIndex dev = device(q, {&data, &table, &lens, cu, out, work});
+    const c10::cuda::CUDAGuard guard(dev);
+    at::Tensor o = out ? *out : fresh({t, h, d}, at::kBFloat16, q);
+    at::Tensor w;
+    if (!work) {
+        w = fresh({(int64_t)lib.workspace_size(t, (int32_t)h, c.kv_heads, (int32_t)d, batch > 0 ? (int32_t)batch : 1)}, at::kByte, q);
+        work = &w;
+    }
+    const int status = lib.paged_attention(
+        static_cast<const uint16_t*>(q.data_ptr()), q.stride(0), q.stride(1), &c, t, (int32_t)h, static_cast<const int32_t*>(table.data_ptr()), table.stride(0), (int32_t)width,
+        static_cast<const int32_t*>(lens.data_ptr()), cu ? static_cast<const int32_t*>(cu->data_ptr()) : nullptr, (int32_t)batch, (int32_t)max_q,
+        scale, static_cast<uint16_t*>(o.data_ptr()), work->data_ptr(), (size_t)work->numel(), c10::cuda::getCurrentCUDAStream(dev).stream());
+    return status ? PyLong_FromLong(status) : THPVariable_Wrap(std::move(o));
+    END_HANDLE_TH_ERRORS
+}
+
+// Addresses of the library's entry points, in the order of Library's members
+PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    TORCH_CHECK_TYPE(n == 6, "expected 6 addresses, got ", n);
+    void* p[6];
+    for (int i = 0; i < 6; ++i) {
+        p[i] = PyLong_AsVoidPtr(a[i]);
+        if (!p[i] && PyErr_Occurred()) throw python_error();
+    }
+    lib = Library{reinterpret_cast<decltype(lib.unit_bytes)>(p[0]),     reinterpret_cast<decltype(lib.qk_norm_rope)>(p[1]),
+                  reinterpret_cast<decltype(lib.kv_write)>(p[2]),       reinterpret_cast<decltype(lib.kv_read)>(p[3]),
+                  reinterpret_cast<decltype(lib.workspace_size)>(p[4]), reinterpret_cast<decltype(lib.paged_attention)>(p[5])};
+    Py_RETURN_NONE;
+    END_HANDLE_TH_ERRORS
+}
+
+#define METHOD(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL, nullptr}
+PyMethodDef methods[] = {METHOD(qk_norm_rope), METHOD(kv_write), METHOD(kv_read), METHOD(paged_attention), METHOD(bind), {}};
+PyModuleDef module{PyModuleDef_HEAD_INIT, "_attention", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
+
+}  // namespace
+
+PyMODINIT_FUNC PyInit__attention() { return PyModule_Create(&module); }

@@ -9,60 +9,35 @@ can be captured in a CUDA graph and replayed with new ones.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 
 import torch
 
 from . import _lib
-from ._lib import BF16, F32, KvCache, check
+from ._lib import check
 
-_CODES = {torch.bfloat16: BF16, torch.float32: F32}
-
-
-def _device(first: torch.Tensor, *others: torch.Tensor | None) -> int:
-    """The CUDA device all of them are on."""
-    d = first.get_device()
-    if d < 0:
-        raise ValueError("expected CUDA tensors")
-    for t in others:
-        if t is not None and t.get_device() != d:
-            raise ValueError(f"tensors on different devices: {first.device} and {t.device}")
-    return d
+_OUT = {torch.bfloat16: True, torch.float32: False}
+_bound = None  # the compiled front end (csrc/attention_torch.cpp), with the library's entry points
 
 
-def _current(device: int):
-    """Makes the device the current one, where it is not already."""
-    return contextlib.nullcontext() if device == torch.cuda.current_device() else torch.cuda.device(device)
+def _front():
+    global _bound
+    if _bound is None:
+        lib = _lib.load()
+        try:
+            from . import _attention
+        except ImportError as e:
+            raise ImportError("marlin_q4/_attention.so is missing or was built for another torch: build it with "
+                              "`python marlin-mlx_b200/build.py` (there is no other path)") from e
+        _attention.bind(*(ctypes.cast(getattr(lib, "marlin_q4_" + f), ctypes.c_void_p).value for f in (
+            "kv_unit_bytes", "qk_norm_rope", "kv_write", "kv_read", "paged_attention_workspace_size", "paged_attention")))
+        _bound = _attention
+    return _bound
 
 
-def _call(device: int, name: str, *args) -> None:
-    """Calls the library on the device's current stream (its last argument), with the device current."""
-    fn = getattr(_lib.load(), name)
-    stream = torch._C._cuda_getCurrentRawStream(device)
-    with _current(device):
-        status = fn(*args, stream)
-    if status:
-        check(status, name)
-
-
-def _heads(t: torch.Tensor, name: str):
-    """Shape and strides of a [tokens, heads, head_dim] operand."""
-    if t.dim() != 3:
-        raise ValueError(f"{name} must be [tokens, heads, head_dim], got {tuple(t.shape)}")
-    if t.dtype not in _CODES:
-        raise TypeError(f"{name} must be bfloat16 or float32, got {t.dtype}")
-    stride = t.stride()
-    if stride[2] != 1:
-        raise ValueError(f"{name}'s features must be contiguous")
-    return t.shape, stride
-
-
-def _int32(t: torch.Tensor, name: str, *shape: int) -> None:
-    if t.dtype is not torch.int32:
-        raise TypeError(f"{name} must be int32, got {t.dtype}")
-    if t.shape != shape or not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous {list(shape)}, got {list(t.shape)}")
+def _unit_bytes(head_dim: int, bits: int) -> int:
+    """marlin_q4_kv_unit_bytes: 16 positions' codes, scales and biases, keys and values; 0 if unsupported."""
+    return 32 * (head_dim * bits // 8 + head_dim // 16) if head_dim in (64, 128, 256) and bits in (4, 8) else 0
 
 
 class KVCache:
@@ -70,21 +45,20 @@ class KVCache:
     bytes] (marlin_q4_kv_cache); groups of 64 features, 4 or 8 bits."""
 
     def __init__(self, data: torch.Tensor, head_dim: int, bits: int = 4):
-        unit = _lib.load().marlin_q4_kv_unit_bytes(head_dim, bits)
+        unit = _unit_bytes(head_dim, bits)
         if unit == 0:
             raise ValueError(f"unsupported head_dim {head_dim} or bits {bits} (64, 128, 256; 4, 8)")
-        if data.dtype != torch.uint8 or data.dim() != 4 or data.shape[3] != unit or not data.is_contiguous():
+        shape = data.shape
+        if data.dtype is not torch.uint8 or len(shape) != 4 or shape[3] != unit or not data.is_contiguous():
             raise ValueError(f"data must be contiguous uint8 [pages, kv_heads, page_size / 16, {unit}]")
         self.data, self.head_dim, self.bits = data, head_dim, bits
-        self.pages, self.kv_heads, self.page_size = data.shape[0], data.shape[1], data.shape[2] * 16
-        self._c = KvCache(data.data_ptr(), self.pages, self.page_size, self.kv_heads, head_dim, bits)
-        self._ref = ctypes.byref(self._c)
+        self.pages, self.kv_heads, self.page_size = shape[0], shape[1], shape[2] * 16
 
     @classmethod
     def empty(cls, pages: int, page_size: int, kv_heads: int, head_dim: int, bits: int = 4,
               device="cuda") -> "KVCache":
         """A pool of zeros: page_size a multiple of 16."""
-        unit = _lib.load().marlin_q4_kv_unit_bytes(head_dim, bits)
+        unit = _unit_bytes(head_dim, bits)
         if unit == 0 or page_size <= 0 or page_size % 16:
             raise ValueError("unsupported head_dim, bits or page_size (64, 128, 256; 4, 8; a multiple of 16)")
         return cls(torch.zeros((pages, kv_heads, page_size // 16, unit), dtype=torch.uint8, device=device), head_dim, bits)
@@ -111,51 +85,30 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: torch.Tensor, k_wei
 
     q [tokens, heads, head_dim] and k [tokens, kv_heads, head_dim], bf16 or f32, may be strided views of a
     fused projection; positions int32 [tokens] or [axes, tokens].  Returns contiguous (q, k) of out_dtype."""
-    (t, h, d), qs = _heads(q, "q")
-    kshape, ks = _heads(k, "k")
-    if q.dtype != k.dtype or out_dtype not in _CODES:
-        raise TypeError("q and k must have one dtype, out_dtype must be bfloat16 or float32")
-    kvh = kshape[1]
-    if kshape[0] != t or kshape[2] != d:
-        raise ValueError(f"k {tuple(k.shape)} does not match q {tuple(q.shape)}")
-    axes = 1 if positions.dim() == 1 else positions.shape[0]
-    _int32(positions, "positions", *((t,) if positions.dim() == 1 else (axes, t)))
-    for w, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
-        if w.dtype is not torch.bfloat16 or w.shape != (d,) or not w.is_contiguous():
-            raise ValueError(f"{name} must be contiguous bfloat16 [{d}]")
-    dev = _device(q, k, q_weight, k_weight, positions, rotary.inv_freq)
-    qo = q.new_empty((t, h, d), dtype=out_dtype)
-    ko = q.new_empty((t, kvh, d), dtype=out_dtype)
-    _call(dev, "marlin_q4_qk_norm_rope", q.data_ptr(), qs[0], qs[1], k.data_ptr(), ks[0], ks[1], _CODES[q.dtype], t, h, kvh, d,
-          q_weight.data_ptr(), k_weight.data_ptr(), eps, positions.data_ptr(), axes, rotary.axes, rotary.inv_freq.data_ptr(),
-          2 * rotary.inv_freq.shape[0], rotary.interleaved, qo.data_ptr(), ko.data_ptr(), _CODES[out_dtype])
-    return qo, ko
+    if out_dtype not in _OUT:
+        raise TypeError("out_dtype must be bfloat16 or float32")
+    r = (_bound or _front()).qk_norm_rope(q, k, q_weight, k_weight, positions, rotary.inv_freq, rotary.interleaved,
+                                          rotary.axes, eps, _OUT[out_dtype])
+    if type(r) is int:
+        check(r, "marlin_q4_qk_norm_rope")
+    return r
 
 
 def kv_write(cache: KVCache, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
     """Quantize k, v [tokens, kv_heads, head_dim] (bf16 or f32) into the cache rows ``slots`` (int32
     [tokens], page * page_size + row; negative: skip the token).  The slots >= 0 must differ."""
-    (t, h, d), ks = _heads(k, "k")
-    _, vs = _heads(v, "v")
-    if h != cache.kv_heads or d != cache.head_dim or k.shape != v.shape or k.dtype != v.dtype:
-        raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} must be [tokens, {cache.kv_heads}, {cache.head_dim}]"
-                         " of one dtype")
-    _int32(slots, "slots", t)
-    dev = _device(cache.data, k, v, slots)
-    _call(dev, "marlin_q4_kv_write", cache._ref, k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1], _CODES[k.dtype],
-          slots.data_ptr(), t)
+    r = (_bound or _front()).kv_write(cache.data, cache.head_dim, cache.bits, k, v, slots)
+    if r:
+        check(r, "marlin_q4_kv_write")
 
 
 def kv_read(cache: KVCache, slots: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """The keys and values of cache rows ``slots`` (int32 [tokens]; negative: zeros) as bf16 [tokens,
     kv_heads, head_dim], bf16(scale * code + bias)."""
-    t = slots.numel()
-    _int32(slots, "slots", t)
-    dev = _device(cache.data, slots)
-    k = slots.new_empty((t, cache.kv_heads, cache.head_dim), dtype=torch.bfloat16)
-    v = slots.new_empty((t, cache.kv_heads, cache.head_dim), dtype=torch.bfloat16)
-    _call(dev, "marlin_q4_kv_read", cache._ref, slots.data_ptr(), t, k.data_ptr(), v.data_ptr())
-    return k, v
+    r = (_bound or _front()).kv_read(cache.data, cache.head_dim, cache.bits, slots)
+    if type(r) is int:
+        check(r, "marlin_q4_kv_read")
+    return r
 
 
 def paged_attention(q: torch.Tensor, cache: KVCache, block_table: torch.Tensor, kv_lens: torch.Tensor,
@@ -168,33 +121,11 @@ def paged_attention(q: torch.Tensor, cache: KVCache, block_table: torch.Tensor, 
     any, or None for one token per sequence.  scale defaults to head_dim ** -0.5.  Rows of ``out`` outside
     every sequence are left as they were.  workspace: uint8 of at least attention_workspace_size bytes; calls
     that may overlap in time (other streams, graphs) need one each.  Without it one is allocated."""
-    (t, h, d), qs = _heads(q, "q")
-    if q.dtype is not torch.bfloat16:
-        raise TypeError(f"q must be bfloat16, got {q.dtype}")
-    if d != cache.head_dim:
-        raise ValueError(f"q's head_dim {d} is not the cache's {cache.head_dim}")
-    if block_table.dtype is not torch.int32 or block_table.dim() != 2:
-        raise ValueError("block_table must be int32 [batch, pages]")
-    batch, width = block_table.shape
-    ts = block_table.stride()
-    if ts[1] != 1 and width > 1:
-        raise ValueError("block_table's rows must be contiguous")
-    _int32(kv_lens, "kv_lens", batch)
-    if cu_q is not None:
-        _int32(cu_q, "cu_q", batch + 1)
-    dev = _device(q, cache.data, block_table, kv_lens, cu_q, out, workspace)
-    if out is None:
-        out = q.new_empty((t, h, d))
-    elif out.dtype is not torch.bfloat16 or out.shape != q.shape or not out.is_contiguous():
-        raise ValueError(f"out must be contiguous bfloat16 {list(q.shape)}")
-    if workspace is None:
-        with _current(dev):
-            size = _lib.load().marlin_q4_paged_attention_workspace_size(t, h, cache.kv_heads, d, max(batch, 1))
-        workspace = q.new_empty(size, dtype=torch.uint8)
-    _call(dev, "marlin_q4_paged_attention", q.data_ptr(), qs[0], qs[1], cache._ref, t, h, block_table.data_ptr(), ts[0], width,
-          kv_lens.data_ptr(), None if cu_q is None else cu_q.data_ptr(), batch, max_q, d ** -0.5 if scale is None else scale,
-          out.data_ptr(), workspace.data_ptr(), workspace.numel())
-    return out
+    r = (_bound or _front()).paged_attention(q, cache.data, cache.head_dim, cache.bits, block_table, kv_lens, cu_q, max_q,
+                                             scale, out, workspace)
+    if type(r) is int:
+        check(r, "marlin_q4_paged_attention")
+    return r
 
 
 def attention_workspace_size(tokens: int, heads: int, kv_heads: int, head_dim: int, batch: int) -> int:

@@ -175,3 +175,40 @@ def test_front_end_refusals():
         mq.paged_attention(q[..., :64], c, table, slots)
     with pytest.raises(ValueError):
         mq.paged_attention(q, c, table.long(), slots)
+
+
+def test_front_end_refuses_what_is_no_tensor_or_of_another_shape():
+    z = torch.zeros
+    c = mq.KVCache(z((2, 2, 1, 16 * 2 * (64 + 8)), dtype=torch.uint8), 128, 4)
+    k, slots, w = z((3, 2, 128), dtype=torch.bfloat16), z(3, dtype=torch.int32), z(128, dtype=torch.bfloat16)
+    q, rot, table = z((3, 4, 128), dtype=torch.bfloat16), mq.Rotary(z(32)), z((3, 2), dtype=torch.int32)
+    for bad in (None, 3, [0.0]):
+        with pytest.raises(TypeError):
+            mq.kv_write(c, bad, k, slots)
+        with pytest.raises(TypeError):
+            mq.kv_read(c, bad)
+        with pytest.raises(TypeError):
+            mq.qk_norm_rope(q, bad, w, w, slots, rot)
+        with pytest.raises(TypeError):
+            mq.paged_attention(q, c, bad, slots)
+    with pytest.raises(ValueError):  # a strided feature axis
+        mq.kv_write(c, z((3, 2, 256), dtype=torch.bfloat16)[..., ::2], k, slots)
+    with pytest.raises(ValueError):
+        mq.kv_write(c, k[0], k[0], slots)
+    with pytest.raises(ValueError):
+        mq.qk_norm_rope(q, k, w, w, slots[0], rot)
+    with pytest.raises(TypeError):
+        mq.qk_norm_rope(q, k, w, w, slots, rot, out_dtype=torch.float16)
+    with pytest.raises(ValueError):
+        mq.paged_attention(q, c, table, slots, slots, 1)  # starts: batch + 1
+    with pytest.raises(ValueError):
+        mq.paged_attention(q, c, table, slots, max_q=1 << 40)
+    with pytest.raises(TypeError):
+        mq.paged_attention(q, c, table, slots, max_q="1")
+    with pytest.raises(ValueError):
+        mq.paged_attention(q, c, table, slots, out=q.float())
+    with pytest.raises(ValueError):
+        mq.paged_attention(q, c, table, slots, workspace=z(1 << 20))
+    c.data = c.data[:, :, :, :-1]  # a pool replaced behind the cache's back
+    with pytest.raises(ValueError):
+        mq.kv_write(c, k, k, slots)
