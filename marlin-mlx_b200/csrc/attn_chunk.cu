@@ -36,7 +36,7 @@ constexpr int kRows = 128;       // rows of a tile (M)
 constexpr int kKeys = 128;       // positions of a step
 constexpr int kSoft = 8;         // softmax warps
 constexpr int kWarpDeq = 8;      // first dequantizing warp
-constexpr uint32_t kItemCost = 2;  // fixed cost of an item (queries, pipeline fill, output), in steps
+constexpr uint32_t kItemCost = 3;  // fixed cost of an item (queries, pipeline fill, output), in steps
 constexpr uint32_t kTmemCols = 512;
 constexpr float kLazy = 10.f;    // log2 of how far a row may outgrow its maximum (f16 holds 2^15) before O is rescaled
 constexpr int kRing = 4;         // steps whose tables may be in use
@@ -373,13 +373,13 @@ __device__ __forceinline__ float4 exponents(const float4* e) {
     const uint4 x = lds128(e);
     return make_float4(__uint_as_float(x.x), __uint_as_float(x.y), __uint_as_float(x.z), __uint_as_float(x.w));
 }
-// N columns of a row of S, -inf from column `seen` on
+// N columns of a row of S, -inf from column `seen` on; `all` (the same for the warp): columns that every row sees
 template <int N>
-__device__ __forceinline__ void load_scores(uint32_t ts, bool mask, int seen, uint32_t (&x)[N]) {
+__device__ __forceinline__ void load_scores(uint32_t ts, int all, int seen, uint32_t (&x)[N]) {
 #pragma unroll
     for (int q = 0; q < N / 32; ++q) tmem_ld32(ts + 32 * q, reinterpret_cast<uint32_t(&)[32]>(x[32 * q]));
     tmem_wait_ld();
-    if (mask) {
+    if (all < N) {
 #pragma unroll
         for (int c = 0; c < N; ++c)
             if (c >= seen) x[c] = 0xff800000u;
@@ -511,9 +511,9 @@ __global__ void __launch_bounds__(ChunkCfg<D, BITS>::THREADS, 1)
             const int nrows = min(kRows, s.n * a.group - it.row0), rr = it.row0 + r;
             bool ok = n == 0 || warp_wait<true>(&qready[busy & 1], (busy >> 1) & 1, abort);
             const float sr = qsr[(busy & 1) * kRows + r];
-            const int lim = r < nrows ? min(s.len, s.len - s.n + rr / a.group + 1) : 0;
+            // rows behind the last one are zeros, see every position and leave no trace
+            const int lim = min(s.len, s.len - s.n + rr / a.group + 1);
             const int low = min(s.len, s.len - s.n + (it.row0 + quarter * 32) / a.group + 1);  // the warp's first row sees least
-            const bool short_tile = quarter * 32 + 32 > nrows;
             float m = -INFINITY, l = 0.f;
             for (int j = 0; j < n; ++j) {
                 const uint32_t gj = base + j, sl = gj % kRing;
@@ -529,7 +529,7 @@ __global__ void __launch_bounds__(ChunkCfg<D, BITS>::THREADS, 1)
                 const float4* ex = expo + sl * 8 + upper * 4;
                 float* xc = xch + (gj & 1) * (2 * kRows);
                 uint32_t x[64];
-                load_scores(ts, pos + 64 > low || short_tile, lim - pos, x);
+                load_scores(ts, low - pos, lim - pos, x);
                 float xm = maximum(x, ex, sr);
                 xc[upper * kRows + r] = xm;
                 pair_barrier(quarter);
