@@ -915,48 +915,60 @@ __global__ void __launch_bounds__(ChunkCfg<D, BITS>::THREADS, 1)
     }
 }
 
-// Joins the rows of cut tiles: block (cut tile, 16-row part), a warp per two rows.
+// Joins the rows of cut tiles: block (cut tile, 8 rows), a warp per row.  What the planning kernel wrote is read
+// while the chunk kernel still runs (it was there before that one's own wait returned); then four partial rows
+// at a time, loaded along with their (M, l).
 template <int D>
 __global__ void __launch_bounds__(256) attn_chunk_join_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ ChunkWork work) {
+    constexpr int AT = 4;
+    const bool any = blockIdx.x < work.head[0];
+    const uint32_t share = work.head[1];
+    const Cut c = any ? work.cuts[blockIdx.x] : Cut{};
+    const SeqSpan s = seq_span(a, c.b);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n = c.c1 - c.c0 + 1;
+    const int r = blockIdx.y * 8 + warp, rr = c.row0 + r;
     pdl_wait();
     pdl_launch_dependents();
-    if (blockIdx.x >= work.head[0]) return;
-    const Cut c = work.cuts[blockIdx.x];
-    const uint32_t share = work.head[1];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n = c.c1 - c.c0 + 1;
-    const SeqSpan s = seq_span(a, c.b);
-    for (int i = 0; i < 2; ++i) {
-        const int r = blockIdx.y * 16 + warp * 2 + i, rr = c.row0 + r;
-        if (rr >= s.n * a.group) continue;
-        auto at = [&](int k) {
-            const uint32_t cta = c.c0 + k;
-            return (int64_t)(2 * cta + (cta * share >= c.at ? 0 : 1)) * kRows + r;
-        };
-        float mx = -INFINITY;
-        for (int k = lane; k < n; k += 32) mx = fmaxf(mx, work.ml[at(k)].x);
+    if (!any || rr >= s.n * a.group) return;
+    float m = -INFINITY, sum = 0.f, acc[D / 32] = {};
+    for (int k0 = 0; k0 < n; k0 += AT) {
+        float2 e[AT], v[AT][D / 64];
 #pragma unroll
-        for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-        if (mx == -INFINITY) mx = 0.f;
-        float sum = 0.f, acc[D / 32] = {};
-#pragma unroll 4
-        for (int k = 0; k < n; ++k) {
-            const float2 e = work.ml[at(k)];
-            const float f = ex2(e.x - mx);
-            sum += f * e.y;
-            const float2* o = reinterpret_cast<const float2*>(work.o + at(k) * D);
+        for (int k = 0; k < AT; ++k) {
+            e[k] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+            for (int q = 0; q < D / 64; ++q) v[k][q] = make_float2(0.f, 0.f);
+            if (k0 + k >= n) continue;
+            const uint32_t cta = c.c0 + k0 + k;
+            const int64_t at = (int64_t)(2 * cta + (cta * share >= c.at ? 0 : 1)) * kRows + r;
+            e[k] = work.ml[at];
+#pragma unroll
+            for (int q = 0; q < D / 64; ++q) v[k][q] = reinterpret_cast<const float2*>(work.o + at * D)[q * 32 + lane];
+        }
+        float mx = m;
+#pragma unroll
+        for (int k = 0; k < AT; ++k) mx = fmaxf(mx, e[k].x);
+        const float mm = mx == -INFINITY ? 0.f : mx, by = ex2(m - mm);
+        m = mx;
+        sum *= by;
+#pragma unroll
+        for (int q = 0; q < D / 32; ++q) acc[q] *= by;
+#pragma unroll
+        for (int k = 0; k < AT; ++k) {
+            const float f = ex2(e[k].x - mm);
+            sum += f * e[k].y;
 #pragma unroll
             for (int q = 0; q < D / 64; ++q) {
-                const float2 v = o[q * 32 + lane];
-                acc[2 * q] += f * v.x;
-                acc[2 * q + 1] += f * v.y;
+                acc[2 * q] += f * v[k][q].x;
+                acc[2 * q + 1] += f * v[k][q].y;
             }
         }
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        uint16_t* y = a.out + ((int64_t)(s.q0 + rr / a.group) * a.heads + c.h * a.group + rr % a.group) * D;
-#pragma unroll
-        for (int q = 0; q < D / 64; ++q)
-            reinterpret_cast<uint32_t*>(y)[q * 32 + lane] = bf16x2_of(acc[2 * q] * inv, acc[2 * q + 1] * inv);
     }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    uint16_t* y = a.out + ((int64_t)(s.q0 + rr / a.group) * a.heads + c.h * a.group + rr % a.group) * D;
+#pragma unroll
+    for (int q = 0; q < D / 64; ++q)
+        reinterpret_cast<uint32_t*>(y)[q * 32 + lane] = bf16x2_of(acc[2 * q] * inv, acc[2 * q + 1] * inv);
 }
 
 template <typename... P, typename... A>
@@ -995,7 +1007,7 @@ cudaError_t run_chunk(const AttnArgs& a, cudaStream_t stream) {
     if (e != cudaSuccess) return e;
     const int64_t cuts = std::min<int64_t>(tiles * a.pool.kv_heads, sms - 1);
     if (cuts < 1) return cudaSuccess;
-    return launch_chunk(attn_chunk_join_kernel<D>, dim3((unsigned)cuts, kRows / 16), 256, 0, a.pdl, stream, a, w);
+    return launch_chunk(attn_chunk_join_kernel<D>, dim3((unsigned)cuts, kRows / 8), 256, 0, a.pdl, stream, a, w);
 }
 
 }  // namespace

@@ -31,6 +31,7 @@ namespace marlin {
 namespace {
 
 constexpr int kWarps = 4;
+constexpr int kStepMaxCtas = 5;  // per SM, the most of any StepCfg
 constexpr int kThreads = kWarps * 32;
 constexpr uint32_t kTileCost = 8;    // fixed cost of a tile (queries, joining the warps), in units
 constexpr uint32_t kMinShare = kTileCost + 2 * kWarps;  // units: one pair per warp
@@ -52,20 +53,17 @@ struct StepCfg {
     static constexpr uint32_t SMEM = OFF_PRE + (kAttnMaxBatch + 1) * 4;
 };
 
-// Workspace: [kAttnMaxBatch + 1] u32 prefix of the work, share (u32), then per slot ROWS (M, l) pairs,
-// then per slot [ROWS][D] partial rows.  Slots 2 c and 2 c + 1 belong to CTA c (its first range, its last).
+// Workspace: per slot ROWS (M, l) pairs, then per slot [ROWS][D] partial rows.  Slots 2 c and 2 c + 1 belong
+// to CTA c (its first range, its last).
 struct StepWork {
-    uint32_t* prefix;
     float2* ml;
     float* o;
 };
-constexpr size_t kStepHead = ((kAttnMaxBatch + 2) * 4 + 255) / 256 * 256;
 __host__ __device__ inline StepWork step_work(float* part, int grid, int rows) {
     uint8_t* p = reinterpret_cast<uint8_t*>(part);
     StepWork w;
-    w.prefix = reinterpret_cast<uint32_t*>(p);
-    w.ml = reinterpret_cast<float2*>(p + kStepHead);
-    w.o = reinterpret_cast<float*>(p + kStepHead + (size_t)2 * grid * rows * 8);
+    w.ml = reinterpret_cast<float2*>(p);
+    w.o = reinterpret_cast<float*>(p + (size_t)2 * grid * rows * 8);
     return w;
 }
 
@@ -74,6 +72,7 @@ __device__ __forceinline__ uint32_t units_of(int len) { return (uint32_t)((len +
 __device__ __forceinline__ uint32_t tile_work(const SeqSpan& s) {
     return s.n > 0 && s.len > 0 ? units_of(s.len) + kTileCost : 0u;
 }
+__device__ __forceinline__ uint32_t share_of(uint32_t total, uint32_t ctas) { return max(kMinShare, (total + ctas - 1) / ctas); }
 
 __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
     uint32_t y;
@@ -171,12 +170,8 @@ __global__ void __launch_bounds__(kThreads, StepCfg<D, BITS, NT>::CTAS) attn_ste
     }
     __syncthreads();
     const uint32_t total = base;
-    const uint32_t share = whole_tiles ? total / a.pool.kv_heads : max(kMinShare, (total + gridDim.x - 1) / gridDim.x);
+    const uint32_t share = whole_tiles ? total / a.pool.kv_heads : share_of(total, gridDim.x);
     const StepWork work = step_work(a.part, gridDim.x, C::ROWS);
-    if (blockIdx.x == 0 && !whole_tiles) {
-        for (int b = tid; b <= a.batch; b += kThreads) work.prefix[b] = pre[b];
-        if (tid == 0) work.prefix[kAttnMaxBatch + 1] = share;
-    }
     const uint64_t w_begin = (uint64_t)(whole_tiles ? (int)blockIdx.x % a.pool.kv_heads : (int)blockIdx.x) * share;
     const uint32_t w_end = (uint32_t)min((uint64_t)total, w_begin + share);
 
@@ -568,30 +563,55 @@ __global__ void __launch_bounds__(kThreads, StepCfg<D, BITS, NT>::CTAS) attn_ste
 
 // Joins the partial rows of tile (sequence, kv head) blockIdx.x, if it was cut.  gridDim.y blocks share its
 // (row, 64 features) parts; in a block 16 lanes take 4 features each, 16 lane groups every 16th partial.
+// Bound: latency.  Where the tile was cut is worked out from the lengths while the step kernel still runs
+// (they were written before its own wait returned), and the first partial rows are loaded along with their
+// (M, l): 131072 positions of 8 heads of 256 features, 4 bits, 3.9 us from the last partial row to the end of
+// the call, 6.0 with these loads one after the other.
 template <int D>
 __global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ AttnArgs a, int grid, int rows) {
-    constexpr int F = 16, GROUPS = 256 / F;
-    __shared__ float wgt[1024];
+    constexpr int F = 16, GROUPS = 256 / F, AHEAD = 8;
+    __shared__ float wgt[kStepMaxCtas * 256];
     __shared__ float4 acc_s[256];
     __shared__ float2 red[8];
+    __shared__ uint2 sums[8];
     const int tid = threadIdx.x;
-    pdl_wait();
-    pdl_launch_dependents();
     const StepWork work = step_work(a.part, grid, rows);
     const int b = blockIdx.x / a.pool.kv_heads, h = blockIdx.x % a.pool.kv_heads;
-    const uint32_t from = work.prefix[b], share = work.prefix[kAttnMaxBatch + 1];
-    const uint32_t vl = (work.prefix[b + 1] - from) / a.pool.kv_heads;
-    if (vl == 0) return;
-    const uint32_t first = from + h * vl, c0 = (first + kTileCost) / share, c1 = (first + vl - 1) / share;
-    if (c0 == c1) return;  // one CTA did all of it
+    uint32_t total = 0, from = 0;
+    for (int i = tid; i < a.batch; i += 256) {
+        const uint32_t v = tile_work(seq_span(a, i)) * (uint32_t)a.pool.kv_heads;
+        total += v;
+        if (i < b) from += v;
+    }
+    total = __reduce_add_sync(0xffffffffu, total);
+    from = __reduce_add_sync(0xffffffffu, from);
+    if (tid % 32 == 0) sums[tid / 32] = make_uint2(total, from);
     const SeqSpan s = seq_span(a, b);
+    __syncthreads();
+    total = from = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) total += sums[i].x, from += sums[i].y;
+    const uint32_t share = share_of(total, grid), vl = tile_work(s);
+    const uint32_t first = from + h * vl, c0 = (first + kTileCost) / share, c1 = (first + max(vl, 1u) - 1) / share;
+    pdl_wait();
+    pdl_launch_dependents();
+    if (vl == 0 || c0 == c1) return;  // nothing, or one CTA did all of it
     const uint32_t n = c1 - c0 + 1;
     auto slot_of = [&](uint32_t i) { return 2 * (c0 + i) + ((uint64_t)(c0 + i) * share >= first ? 0 : 1); };
     const int f = tid % F, grp = tid / F;
     for (int part = blockIdx.y; part < s.n * a.group * (D / 64); part += gridDim.y) {
         const int row = part / (D / 64), fo = part % (D / 64) * 16 + f;
-        float mx = -INFINITY;
-        for (uint32_t i = tid; i < n; i += 256) mx = fmaxf(mx, work.ml[slot_of(i) * rows + row].x);
+        auto partial = [&](uint32_t i) { return reinterpret_cast<const float4*>(work.o)[((int64_t)slot_of(i) * rows + row) * (D / 4) + fo]; };
+        float2 e0 = make_float2(-INFINITY, 0.f);
+        if (tid < n) e0 = work.ml[slot_of(tid) * rows + row];
+        float4 v[AHEAD];
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k) {
+            v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (grp + k * GROUPS < n) v[k] = partial(grp + k * GROUPS);
+        }
+        float mx = e0.x;
+        for (uint32_t i = tid + 256; i < n; i += 256) mx = fmaxf(mx, work.ml[slot_of(i) * rows + row].x);
 #pragma unroll
         for (int o = 16; o; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
         if (tid % 32 == 0) red[tid / 32].x = mx;
@@ -602,7 +622,7 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ 
         if (mx == -INFINITY) mx = 0.f;
         float sum = 0.f;
         for (uint32_t i = tid; i < n; i += 256) {
-            const float2 e = work.ml[slot_of(i) * rows + row];
+            const float2 e = i < 256 ? e0 : work.ml[slot_of(i) * rows + row];
             const float w = ex2(e.x - mx);
             wgt[i] = w;
             sum += w * e.y;
@@ -615,18 +635,19 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ 
 #pragma unroll
         for (int i = 0; i < 8; ++i) sum += red[i].y;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        auto add = [&](float w, const float4& x) { acc.x += w * x.x, acc.y += w * x.y, acc.z += w * x.z, acc.w += w * x.w; };
+#pragma unroll
+        for (int k = 0; k < AHEAD; ++k)
+            if (grp + k * GROUPS < n) add(wgt[grp + k * GROUPS], v[k]);
 #pragma unroll 8
-        for (uint32_t i = grp; i < n; i += GROUPS) {
-            const float4 v = reinterpret_cast<const float4*>(work.o)[((int64_t)slot_of(i) * rows + row) * (D / 4) + fo];
-            const float w = wgt[i];
-            acc.x += w * v.x, acc.y += w * v.y, acc.z += w * v.z, acc.w += w * v.w;
-        }
+        for (uint32_t i = grp + AHEAD * GROUPS; i < n; i += GROUPS) add(wgt[i], partial(i));
         acc_s[tid] = acc;
         __syncthreads();
         if (grp == 0) {
+#pragma unroll
             for (int i = 1; i < GROUPS; ++i) {
-                const float4 v = acc_s[i * F + f];
-                acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
+                const float4 x = acc_s[i * F + f];
+                acc.x += x.x, acc.y += x.y, acc.z += x.z, acc.w += x.w;
             }
             const float inv = sum == 0.f ? 0.f : 1.f / sum;
             uint16_t* y = a.out + ((int64_t)(s.q0 + row / a.group) * a.heads + h * a.group + row % a.group) * D + fo * 4;
@@ -651,7 +672,6 @@ cudaError_t launch_attn(void (*kernel)(P...), dim3 grid, int threads, uint32_t s
     return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
 }
 
-constexpr int kStepMaxCtas = 5;  // per SM, the most of any StepCfg
 
 template <int D, int BITS, int NT>
 cudaError_t run_step(const AttnArgs& a, cudaStream_t stream) {
@@ -681,7 +701,7 @@ cudaError_t run_rows(const AttnArgs& a, cudaStream_t stream) {
 bool step_applies(const AttnArgs& a) { return (int64_t)a.max_q * a.group <= 16; }
 
 size_t step_workspace_bytes(int dim) {
-    return kStepHead + (size_t)2 * device_num_sms() * kStepMaxCtas * 16 * (dim * 4 + 8);
+    return (size_t)2 * device_num_sms() * kStepMaxCtas * 16 * (dim * 4 + 8);
 }
 
 cudaError_t launch_attn_step(const AttnArgs& a, cudaStream_t stream) {
