@@ -46,7 +46,7 @@ struct Item {
     int b, h, row0;  // sequence, kv head, first row of the tile
     int k0, k1;      // steps
     int slot;        // partial rows, -1: the whole tile
-    int cta, pad;
+    int pad[2];
 };
 struct Cut {         // a tile of several items: CTAs c0 .. c1, its place in the order of work
     int b, h, row0, c0, c1;
@@ -148,18 +148,21 @@ __global__ void __launch_bounds__(1024) attn_plan_kernel(const __grid_constant__
         row0 = (i - first_tile[lo]) * kRows;
         return tile_steps(span[lo], row0, a.group);
     };
-    uint32_t total = 0;
-    for (int i0 = 0; i0 < tiles; i0 += 1024) {
-        int b, row0;
-        block_scan(make_uint3(i0 + tid < tiles ? tile_of(i0 + tid, b, row0) + kItemCost : 0u, 0, 0), tmp, all);
-        total += all.x;
-    }
-    total *= a.pool.kv_heads;
-    const uint32_t share = max(kItemCost + 2, (total + ctas - 1) / ctas);
-    uint32_t place = 0, items = 0, cuts = 0;
     const int everything = tiles * a.pool.kv_heads;
+    auto share_of = [&](uint32_t total) { return max(kItemCost + 2, (total + ctas - 1) / ctas); };
+    uint32_t share = 1;
+    if (everything > 1024) {
+        uint32_t total = 0;
+        for (int i0 = 0; i0 < tiles; i0 += 1024) {
+            int b, row0;
+            block_scan(make_uint3(i0 + tid < tiles ? tile_of(i0 + tid, b, row0) + kItemCost : 0u, 0, 0), tmp, all);
+            total += all.x;
+        }
+        share = share_of(total * a.pool.kv_heads);
+    }
+    uint32_t place = 0, items = 0, cuts = 0;
     for (int i0 = 0; i0 < everything; i0 += 1024) {
-        const int i = i0 + tid, h = i / max(tiles, 1);
+        const int i = i0 + tid, h = i / tiles;
         int b = 0, row0 = 0;
         uint32_t steps = 0;
         const bool live = i < everything;
@@ -167,10 +170,12 @@ __global__ void __launch_bounds__(1024) attn_plan_kernel(const __grid_constant__
         const uint32_t len = live ? steps + kItemCost : 0u;
         const uint32_t p = place + block_scan(make_uint3(len, 0, 0), tmp, all).x;
         place += all.x;
-        // the CTAs that hold steps of it (the fixed cost goes to the first)
-        const uint32_t from = p + kItemCost, c0 = steps ? from / share : p / share, c1 = steps ? (p + len - 1) / share : c0;
-        const uint32_t n = live ? c1 - c0 + 1 : 0u;
+        if (everything <= 1024) share = share_of(all.x);
+        // the CTAs that hold steps of it (the fixed cost goes to the first), and the last of the tile before
+        const uint32_t from = p + kItemCost, c1 = (p + max(len, 1u) - 1) / share, c0 = steps ? from / share : c1;
+        const uint32_t n = live ? c1 - c0 + 1 : 0u, next = p ? (p - 1) / share + 1 : 0u;
         const uint3 o = block_scan(make_uint3(n, n > 1 ? 1u : 0u, 0), tmp, all);
+        for (uint32_t c = next; live && c <= c0; ++c) w.first[c] = (int)(items + o.x);
         for (uint32_t j = 0; j < n; ++j) {
             const uint32_t c = c0 + j;
             Item it{};
@@ -180,25 +185,17 @@ __global__ void __launch_bounds__(1024) attn_plan_kernel(const __grid_constant__
             it.k0 = steps ? (int)(max(c * share, from) - from) : 0;
             it.k1 = steps ? (int)(min((c + 1) * share, p + len) - from) : 0;
             it.slot = n > 1 ? (int)(2 * c + (c * share >= p ? 0 : 1)) : -1;
-            it.cta = (int)c;
             w.items[items + o.x + j] = it;
+            if (j) w.first[c] = (int)(items + o.x + j);
         }
         if (n > 1) w.cuts[cuts + o.y] = Cut{b, h, row0, (int)c0, (int)c1, p};
         items += all.x;
         cuts += all.y;
     }
-    __syncthreads();
-    for (uint32_t i = tid; i < items; i += 1024) {
-        const int c = w.items[i].cta, before = i ? w.items[i - 1].cta : -1;
-        for (int k = before + 1; k <= c; ++k) w.first[k] = (int)i;
-        if (i == items - 1)
-            for (int k = c + 1; k <= ctas; ++k) w.first[k] = (int)items;
-    }
+    for (uint32_t c = (place ? (place - 1) / share + 1 : 0u) + tid; c <= (uint32_t)ctas; c += 1024) w.first[c] = (int)items;
     if (tid == 0) {
         w.head[0] = cuts;
         w.head[1] = share;
-        if (items == 0)
-            for (int k = 0; k <= ctas; ++k) w.first[k] = 0;
     }
 }
 
@@ -916,11 +913,11 @@ __global__ void __launch_bounds__(ChunkCfg<D, BITS>::THREADS, 1)
 }
 
 // Joins the rows of cut tiles: block (cut tile, 8 rows), a warp per row.  What the planning kernel wrote is read
-// while the chunk kernel still runs (it was there before that one's own wait returned); then four partial rows
+// while the chunk kernel still runs (it was there before that one's own wait returned); then two partial rows
 // at a time, loaded along with their (M, l).
 template <int D>
 __global__ void __launch_bounds__(256) attn_chunk_join_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ ChunkWork work) {
-    constexpr int AT = 4;
+    constexpr int AT = 2;  // most cut tiles have two parts
     const bool any = blockIdx.x < work.head[0];
     const uint32_t share = work.head[1];
     const Cut c = any ? work.cuts[blockIdx.x] : Cut{};
