@@ -162,20 +162,28 @@ __global__ void __launch_bounds__(1024) attn_plan_kernel(const __grid_constant__
     }
     uint32_t place = 0, items = 0, cuts = 0;
     for (int i0 = 0; i0 < everything; i0 += 1024) {
-        const int i = i0 + tid, h = i / tiles;
-        int b = 0, row0 = 0;
-        uint32_t steps = 0;
-        const bool live = i < everything;
-        if (live) steps = tile_of(i - h * tiles, b, row0);
-        const uint32_t len = live ? steps + kItemCost : 0u;
+        const int i = i0 + tid;
+        int b = 0, row0 = 0, h = 0;
+        uint32_t steps = 0, len = 0;
+        if (i < everything) {
+            h = i / tiles;
+            steps = tile_of(i - h * tiles, b, row0);
+            len = steps + kItemCost;
+        }
         const uint32_t p = place + block_scan(make_uint3(len, 0, 0), tmp, all).x;
         place += all.x;
         if (everything <= 1024) share = share_of(all.x);
         // the CTAs that hold steps of it (the fixed cost goes to the first), and the last of the tile before
-        const uint32_t from = p + kItemCost, c1 = (p + max(len, 1u) - 1) / share, c0 = steps ? from / share : c1;
-        const uint32_t n = live ? c1 - c0 + 1 : 0u, next = p ? (p - 1) / share + 1 : 0u;
+        const uint32_t from = p + kItemCost;
+        uint32_t c0 = 0, c1 = 0, n = 0, next = 0;
+        if (len) {
+            c1 = (p + len - 1) / share;
+            c0 = steps ? from / share : c1;
+            n = c1 - c0 + 1;
+            next = p ? (p - 1) / share + 1 : 0u;
+        }
         const uint3 o = block_scan(make_uint3(n, n > 1 ? 1u : 0u, 0), tmp, all);
-        for (uint32_t c = next; live && c <= c0; ++c) w.first[c] = (int)(items + o.x);
+        for (uint32_t c = next; n && c <= c0; ++c) w.first[c] = (int)(items + o.x);
         for (uint32_t j = 0; j < n; ++j) {
             const uint32_t c = c0 + j;
             Item it{};
