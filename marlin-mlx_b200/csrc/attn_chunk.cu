@@ -42,7 +42,7 @@ constexpr float kLazy = 10.f;    // log2 of how far a row may outgrow its maximu
 constexpr int kRing = 4;         // steps whose tables may be in use
 
 
-struct Item {
+struct alignas(16) Item {
     int b, h, row0;  // sequence, kv head, first row of the tile
     int k0, k1;      // steps
     int slot;        // partial rows, -1: the whole tile
@@ -88,38 +88,28 @@ __device__ __forceinline__ uint32_t tile_steps(const SeqSpan& s, int row0, int g
     return seen <= 0 ? 0u : (uint32_t)((seen + kKeys - 1) / kKeys);
 }
 
-// Exclusive prefix sums over the 1024 threads of the block of three values at once; `all` returns the
-// totals.
-__device__ __forceinline__ uint3 block_scan(uint3 v, uint3 (&tmp)[32], uint3& all) {
+// Exclusive prefix sum over the 1024 threads of the block; `all` returns the total.  (Not inlined: the planning
+// kernel runs once through its code, so what it takes is mostly the fetching of it.)
+__device__ __noinline__ uint32_t block_scan(uint32_t v, uint32_t* tmp, uint32_t& all) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    uint3 x = v;
+    uint32_t x = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t a = __shfl_up_sync(0xffffffffu, x.x, o), b = __shfl_up_sync(0xffffffffu, x.y, o),
-                       c = __shfl_up_sync(0xffffffffu, x.z, o);
-        if (lane >= o) x.x += a, x.y += b, x.z += c;
+        const uint32_t a = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += a;
     }
     __syncthreads();
     if (lane == 31) tmp[warp] = x;
     __syncthreads();
-    uint3 w = tmp[lane];
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t a = __shfl_up_sync(0xffffffffu, w.x, o), b = __shfl_up_sync(0xffffffffu, w.y, o),
-                       c = __shfl_up_sync(0xffffffffu, w.z, o);
-        if (lane >= o) w.x += a, w.y += b, w.z += c;
-    }
-    all = make_uint3(__shfl_sync(0xffffffffu, w.x, 31), __shfl_sync(0xffffffffu, w.y, 31), __shfl_sync(0xffffffffu, w.z, 31));
-    const int from = (warp + 31) & 31;
-    uint3 before = make_uint3(__shfl_sync(0xffffffffu, w.x, from), __shfl_sync(0xffffffffu, w.y, from), __shfl_sync(0xffffffffu, w.z, from));
-    if (warp == 0) before = make_uint3(0, 0, 0);
-    return make_uint3(x.x - v.x + before.x, x.y - v.y + before.y, x.z - v.z + before.z);
+    const uint32_t w = tmp[lane];
+    all = __reduce_add_sync(0xffffffffu, w);
+    return x - v + __reduce_add_sync(0xffffffffu, lane < warp ? w : 0u);
 }
 
 // One block lays out the items.
 __global__ void __launch_bounds__(1024) attn_plan_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ ChunkWork w,
                                                          int64_t tiles_cap, int ctas) {
-    __shared__ uint3 tmp[32];
+    __shared__ uint32_t tmp[32];
     __shared__ int first_tile[kAttnMaxBatch + 1];
     __shared__ SeqSpan span[kAttnMaxBatch];
     const int tid = threadIdx.x;
@@ -130,9 +120,9 @@ __global__ void __launch_bounds__(1024) attn_plan_kernel(const __grid_constant__
         s = seq_span(a, tid);
         span[tid] = s;
     }
-    uint3 all;
-    const uint32_t at = block_scan(make_uint3((s.n * a.group + kRows - 1) / kRows, 0, 0), tmp, all).x;
-    const uint32_t ntiles = all.x;
+    uint32_t all;
+    const uint32_t at = block_scan((s.n * a.group + kRows - 1) / kRows, tmp, all);
+    const uint32_t ntiles = all;
     if (tid < a.batch) first_tile[tid] = (int)at;
     __syncthreads();
     // starts that overlap could ask for more tiles than the tokens fill
@@ -155,8 +145,8 @@ __global__ void __launch_bounds__(1024) attn_plan_kernel(const __grid_constant__
         uint32_t total = 0;
         for (int i0 = 0; i0 < tiles; i0 += 1024) {
             int b, row0;
-            block_scan(make_uint3(i0 + tid < tiles ? tile_of(i0 + tid, b, row0) + kItemCost : 0u, 0, 0), tmp, all);
-            total += all.x;
+            block_scan(i0 + tid < tiles ? tile_of(i0 + tid, b, row0) + kItemCost : 0u, tmp, all);
+            total += all;
         }
         share = share_of(total * a.pool.kv_heads);
     }
@@ -170,9 +160,9 @@ __global__ void __launch_bounds__(1024) attn_plan_kernel(const __grid_constant__
             steps = tile_of(i - h * tiles, b, row0);
             len = steps + kItemCost;
         }
-        const uint32_t p = place + block_scan(make_uint3(len, 0, 0), tmp, all).x;
-        place += all.x;
-        if (everything <= 1024) share = share_of(all.x);
+        const uint32_t p = place + block_scan(len, tmp, all);
+        place += all;
+        if (everything <= 1024) share = share_of(all);
         // the CTAs that hold steps of it (the fixed cost goes to the first), and the last of the tile before
         const uint32_t from = p + kItemCost;
         uint32_t c0 = 0, c1 = 0, n = 0, next = 0;
@@ -182,8 +172,9 @@ __global__ void __launch_bounds__(1024) attn_plan_kernel(const __grid_constant__
             n = c1 - c0 + 1;
             next = p ? (p - 1) / share + 1 : 0u;
         }
-        const uint3 o = block_scan(make_uint3(n, n > 1 ? 1u : 0u, 0), tmp, all);
-        for (uint32_t c = next; n && c <= c0; ++c) w.first[c] = (int)(items + o.x);
+        // items below, cut tiles above (1024 tiles make fewer than 1024 + CTAs items)
+        const uint32_t o = block_scan(n + (n > 1 ? 0x10000u : 0u), tmp, all), oi = items + (o & 0xffffu);
+        for (uint32_t c = next; n && c <= c0; ++c) w.first[c] = (int)oi;
         for (uint32_t j = 0; j < n; ++j) {
             const uint32_t c = c0 + j;
             Item it{};
@@ -193,12 +184,14 @@ __global__ void __launch_bounds__(1024) attn_plan_kernel(const __grid_constant__
             it.k0 = steps ? (int)(max(c * share, from) - from) : 0;
             it.k1 = steps ? (int)(min((c + 1) * share, p + len) - from) : 0;
             it.slot = n > 1 ? (int)(2 * c + (c * share >= p ? 0 : 1)) : -1;
-            w.items[items + o.x + j] = it;
-            if (j) w.first[c] = (int)(items + o.x + j);
+            const int4* two = reinterpret_cast<const int4*>(&it);
+            reinterpret_cast<int4*>(w.items + oi + j)[0] = two[0];
+            reinterpret_cast<int4*>(w.items + oi + j)[1] = two[1];
+            if (j) w.first[c] = (int)(oi + j);
         }
-        if (n > 1) w.cuts[cuts + o.y] = Cut{b, h, row0, (int)c0, (int)c1, p};
-        items += all.x;
-        cuts += all.y;
+        if (n > 1) w.cuts[cuts + (o >> 16)] = Cut{b, h, row0, (int)c0, (int)c1, p};
+        items += all & 0xffffu;
+        cuts += all >> 16;
     }
     for (uint32_t c = (place ? (place - 1) / share + 1 : 0u) + tid; c <= (uint32_t)ctas; c += 1024) w.first[c] = (int)items;
     if (tid == 0) {
