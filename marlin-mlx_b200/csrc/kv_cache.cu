@@ -181,17 +181,24 @@ __global__ void __launch_bounds__(256) kv_write_kernel(KvPool c, const void* __r
         else
             load8(k, t * k_ts + h * k_hs + g * 64 + lane8 * 8, BF16_IN, x);
     }
-    const int64_t slot = valid ? slots[t] : -1;
-    const int64_t unit = slot / kKvRows;
+    const int slot = valid ? slots[t] : -1;
+    const uint32_t unit = (uint32_t)slot / kKvRows;  // 32-bit quotients: 64-bit ones were a third of the instructions
     bool put = slot >= 0;
     if (put && unit >= c.pages * c.page_units) {
         put = false;
         if (lane8 == 0) record_device_error(kDevErrBadIndex);
     }
     float lo = INFINITY, hi = 0.0f;
+    if (!BF16_IN) {
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+            const uint32_t two = pack_bf16x2(x[i], x[i + 1]);
+            x[i] = __uint_as_float(two << 16);
+            x[i + 1] = __uint_as_float(two & 0xffff0000u);
+        }
+    }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        if (!BF16_IN) x[i] = bf16_round(x[i]);
         lo = fminf(lo, x[i]);
         hi = fmaxf(hi, x[i]);
     }
@@ -222,7 +229,7 @@ __global__ void __launch_bounds__(256) kv_write_kernel(KvPool c, const void* __r
             const float q = fminf(fmaxf(divide(__fsub_rn(x[i], bias), scale, inv), 0.0f), kTop);
             // ties away from zero for q >= 0: floor(q + 1/2), the sum rounded down so that it passes no
             // integer; adding 2^23, rounded down, leaves the floor in the low bits
-            code[i] = __float_as_uint(__fadd_rd(__fadd_rd(q, 0.5f), 8388608.0f)) & 255u;
+            code[i] = __float_as_uint(__fadd_rd(__fadd_rd(q, 0.5f), 8388608.0f));  // the lowest byte counts
         }
     } else {
         scale = fmaxf(__fdiv_rn(__fsub_rn(hi, lo), kTop), 1e-7f);
@@ -242,19 +249,19 @@ __global__ void __launch_bounds__(256) kv_write_kernel(KvPool c, const void* __r
         }
     }
     if (!put) return;
-    const int r = (int)(slot % kKvRows);
-    const int64_t page = unit / c.page_units;
-    uint8_t* u = c.data + ((page * c.kv_heads + h) * c.page_units + unit % c.page_units) * (int64_t)(32 * (rb + 4 * groups));
-    const int j = (g * 64 + lane8 * 8) * BITS / 8;
+    const uint32_t r = (uint32_t)slot % kKvRows, page = unit / (uint32_t)c.page_units;
+    uint8_t* u = c.data + (((int64_t)page * c.kv_heads + h) * c.page_units + (unit - page * c.page_units)) * (32 * (rb + 4 * groups));
+    const uint32_t j = (uint32_t)(g * 64 + lane8 * 8) * BITS / 8;
     uint8_t* dst = u + (isv ? kv_value_code(r, j, rb, groups) : kv_key_code(r, j, rb));
     if (BITS == 4) {
         uint32_t word = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) word |= code[i] << (4 * i);
+        for (int i = 0; i < 8; ++i) word |= (code[i] & 15u) << (4 * i);
         *reinterpret_cast<uint32_t*>(dst) = word;
     } else {
-        *reinterpret_cast<uint2*>(dst) = make_uint2(code[0] | code[1] << 8 | code[2] << 16 | code[3] << 24,
-                                                    code[4] | code[5] << 8 | code[6] << 16 | code[7] << 24);
+        *reinterpret_cast<uint2*>(dst) = make_uint2(
+            __byte_perm(__byte_perm(code[0], code[1], 0x0040), __byte_perm(code[2], code[3], 0x0040), 0x5410),
+            __byte_perm(__byte_perm(code[4], code[5], 0x0040), __byte_perm(code[6], code[7], 0x0040), 0x5410));
     }
     if (lane8 == 0)
         *reinterpret_cast<uint32_t*>(u + (isv ? kv_value_pair(r, g, rb, groups) : kv_key_pair(r, g, rb, groups))) =
@@ -277,13 +284,13 @@ __global__ void __launch_bounds__(256) kv_read_kernel(KvPool c, const int32_t* _
     const int it = i - tb * per, ch = it & (chunks - 1), h = it >> (lc + 1);
     const bool isv = (it >> lc) & 1;
     const int64_t th = t * c.kv_heads + h;
-    const int64_t slot = slots[t], unit = slot / kKvRows;
+    const int slot = slots[t];
+    const uint32_t unit = (uint32_t)slot / kKvRows;
     uint4 o = make_uint4(0u, 0u, 0u, 0u);
     if (slot >= 0 && unit < c.pages * c.page_units) {
-        const int r = (int)(slot % kKvRows), g = ch / 8, j = ch * BITS;
-        const int64_t page = unit / c.page_units;
+        const uint32_t r = (uint32_t)slot % kKvRows, g = ch / 8, j = ch * BITS, page = unit / (uint32_t)c.page_units;
         const uint8_t* u =
-            c.data + ((page * c.kv_heads + h) * c.page_units + unit % c.page_units) * (int64_t)(32 * (rb + 4 * groups));
+            c.data + (((int64_t)page * c.kv_heads + h) * c.page_units + (unit - page * c.page_units)) * (32 * (rb + 4 * groups));
         const uint8_t* src = u + (isv ? kv_value_code(r, j, rb, groups) : kv_key_code(r, j, rb));
         const uint32_t pair = *reinterpret_cast<const uint32_t*>(
             u + (isv ? kv_value_pair(r, g, rb, groups) : kv_key_pair(r, g, rb, groups)));
@@ -297,7 +304,10 @@ __global__ void __launch_bounds__(256) kv_read_kernel(KvPool c, const int32_t* _
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const uint32_t q = i < 2 ? w.x : w.y;
-                const uint32_t two = pack_bf16x2((float)((q >> (16 * (i & 1))) & 255u), (float)((q >> (16 * (i & 1) + 8)) & 255u));
+                // a byte under the exponent of 2^23 is the code plus 2^23
+                const float x = __uint_as_float(__byte_perm(q, 0x4B000000u, i & 1 ? 0x7552 : 0x7550)) - 8388608.0f;
+                const float y = __uint_as_float(__byte_perm(q, 0x4B000000u, i & 1 ? 0x7553 : 0x7551)) - 8388608.0f;
+                const uint32_t two = pack_bf16x2(x, y);
                 p[i] = bf16x2_fma(two, s2, b2);
             }
             o = make_uint4(p[0], p[1], p[2], p[3]);

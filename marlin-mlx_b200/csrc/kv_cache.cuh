@@ -25,18 +25,18 @@ constexpr int kv_row_bytes(int dim, int bits) { return dim * bits / 8; }
 constexpr int kv_unit_bytes(int dim, int bits) { return kKvRows * 2 * (kv_row_bytes(dim, bits) + 4 * (dim / 64)); }
 
 // Byte offsets inside a unit; rb = row bytes, j = byte within the row's codes, groups = dim / 64.
-__host__ __device__ constexpr int kv_key_code(int r, int j, int rb) {
-    const int p = rb < 64 ? rb : 64;
+__host__ __device__ constexpr uint32_t kv_key_code(uint32_t r, uint32_t j, uint32_t rb) {
+    const uint32_t p = rb < 64 ? rb : 64;
     return (j / p) * (p * kKvRows) + r * p + j % p;
 }
-__host__ __device__ constexpr int kv_key_pair(int r, int g, int rb, int groups) {
+__host__ __device__ constexpr uint32_t kv_key_pair(uint32_t r, uint32_t g, uint32_t rb, uint32_t groups) {
     return kKvRows * rb + (r * groups + g) * 4;
 }
-__host__ __device__ constexpr int kv_value_code(int r, int j, int rb, int groups) {
-    const int c = j / 16;
+__host__ __device__ constexpr uint32_t kv_value_code(uint32_t r, uint32_t j, uint32_t rb, uint32_t groups) {
+    const uint32_t c = j / 16;
     return kKvRows * (rb + 4 * groups) + ((c / 2) * 32 + (r % 2 + 2 * (r / 8)) * 8 + (c % 2) * 4 + (r / 2) % 4) * 16 + j % 16;
 }
-__host__ __device__ constexpr int kv_value_pair(int r, int g, int rb, int groups) {
+__host__ __device__ constexpr uint32_t kv_value_pair(uint32_t r, uint32_t g, uint32_t rb, uint32_t groups) {
     return kKvRows * (2 * rb + 4 * groups) + (r * groups + g) * 4;
 }
 
