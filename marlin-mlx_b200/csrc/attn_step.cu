@@ -68,9 +68,13 @@ __host__ __device__ inline StepWork step_work(float* part, int grid, int rows) {
 }
 
 __device__ __forceinline__ uint32_t units_of(int len) { return (uint32_t)((len + kKvRows - 1) / kKvRows); }
+// How the work is cut: into equal shares; a CTA per tile; or into shares of kMinShare, tiles starting at one
+// (where the longest lengths that the table can hold leave CTAs enough for that: no CTA works on two tiles).
+enum : int { kEven, kWholeTiles, kAligned };
 // one tile per (sequence with new tokens and positions, kv head)
-__device__ __forceinline__ uint32_t tile_work(const SeqSpan& s) {
-    return s.n > 0 && s.len > 0 ? units_of(s.len) + kTileCost : 0u;
+__device__ __forceinline__ uint32_t tile_work(const SeqSpan& s, int mode) {
+    const uint32_t v = s.n > 0 && s.len > 0 ? units_of(s.len) + kTileCost : 0u;
+    return mode == kAligned ? (v + kMinShare - 1) / kMinShare * kMinShare : v;
 }
 __device__ __forceinline__ uint32_t share_of(uint32_t total, uint32_t ctas) { return max(kMinShare, (total + ctas - 1) / ctas); }
 
@@ -106,7 +110,8 @@ __device__ __forceinline__ float pair_scale(uint32_t w) { return __uint_as_float
 __device__ __forceinline__ float pair_bias(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
 
 template <int D, int BITS, int NT>
-__global__ void __launch_bounds__(kThreads, StepCfg<D, BITS, NT>::CTAS) attn_step_kernel(const __grid_constant__ AttnArgs a, int whole_tiles) {
+__global__ void __launch_bounds__(kThreads, StepCfg<D, BITS, NT>::CTAS) attn_step_kernel(const __grid_constant__ AttnArgs a, int mode) {
+    const bool whole_tiles = mode == kWholeTiles;
     using C = StepCfg<D, BITS, NT>;
     constexpr int G = C::G;
     extern __shared__ __align__(128) uint8_t smem[];
@@ -138,14 +143,14 @@ __global__ void __launch_bounds__(kThreads, StepCfg<D, BITS, NT>::CTAS) attn_ste
         if (s.len == 0 && (int)blockIdx.x % a.pool.kv_heads == 0)
             for (int64_t i = tid; i < (int64_t)s.n * a.heads * D / 8; i += kThreads)
                 reinterpret_cast<uint4*>(a.out + (int64_t)s.q0 * a.heads * D)[i] = make_uint4(0u, 0u, 0u, 0u);
-        base = tile_work(s) * (uint32_t)a.pool.kv_heads;
+        base = tile_work(s, mode) * (uint32_t)a.pool.kv_heads;
     }
     for (int b0 = 0; b0 < a.batch && !whole_tiles; b0 += kThreads) {
         const int b = b0 + tid;
         uint32_t v = 0;
         if (b < a.batch) {
             const SeqSpan s = seq_span(a, b);
-            v = tile_work(s) * (uint32_t)a.pool.kv_heads;
+            v = tile_work(s, mode) * (uint32_t)a.pool.kv_heads;
             if (s.len == 0 && b % gridDim.x == blockIdx.x)  // no position to attend to: zero rows
                 for (int64_t i = 0; i < (int64_t)s.n * a.heads * D / 8; ++i)
                     reinterpret_cast<uint4*>(a.out + (int64_t)s.q0 * a.heads * D)[i] = make_uint4(0u, 0u, 0u, 0u);
@@ -170,7 +175,7 @@ __global__ void __launch_bounds__(kThreads, StepCfg<D, BITS, NT>::CTAS) attn_ste
     }
     __syncthreads();
     const uint32_t total = base;
-    const uint32_t share = whole_tiles ? total / a.pool.kv_heads : share_of(total, gridDim.x);
+    const uint32_t share = whole_tiles ? total / a.pool.kv_heads : mode == kAligned ? kMinShare : share_of(total, gridDim.x);
     const StepWork work = step_work(a.part, gridDim.x, C::ROWS);
     const uint64_t w_begin = (uint64_t)(whole_tiles ? (int)blockIdx.x % a.pool.kv_heads : (int)blockIdx.x) * share;
     const uint32_t w_end = (uint32_t)min((uint64_t)total, w_begin + share);
@@ -185,11 +190,11 @@ __global__ void __launch_bounds__(kThreads, StepCfg<D, BITS, NT>::CTAS) attn_ste
         }
         const int b = whole_tiles ? only : lo;
         const SeqSpan s = seq_span(a, b);
-        const uint32_t nu = units_of(s.len), vl = nu + kTileCost;
+        const uint32_t nu = units_of(s.len), vl = tile_work(s, mode);
         const uint32_t in = w0 - pre[lo];
         const int h = (int)(in / vl);
         const uint32_t v0 = in - h * vl, v1 = min(vl, v0 + (w_end - w0));
-        const int u0 = (int)(max(v0, kTileCost) - kTileCost), u1 = (int)(max(v1, kTileCost) - kTileCost);
+        const int u0 = (int)(max(v0, kTileCost) - kTileCost), u1 = (int)min(nu, max(v1, kTileCost) - kTileCost);
         const bool whole = u0 == 0 && u1 == (int)nu;
         const int slot = 2 * (int)blockIdx.x + (w0 == (uint32_t)w_begin ? 0 : 1);
         w0 += v1 - v0;
@@ -197,6 +202,18 @@ __global__ void __launch_bounds__(kThreads, StepCfg<D, BITS, NT>::CTAS) attn_ste
         const int nrows = s.n * a.group;  // at most ROWS
         // row r sees the positions below len - n + token + 1
         const int first_seen = min(s.len, s.len - s.n + 1);
+
+        // the warp's query rows: warp, warp + 4, ...
+        constexpr int E = D / 32, QROWS = C::ROWS / kWarps;
+        uint32_t raw[QROWS][E / 2];
+#pragma unroll
+        for (int i = 0; i < QROWS; ++i) {
+            const int rr = min(warp + i * kWarps, nrows - 1);
+            const uint32_t* src_q = reinterpret_cast<const uint32_t*>(a.q + (int64_t)(s.q0 + rr / a.group) * a.q_ts +
+                                                                      (int64_t)(h * a.group + rr % a.group) * a.q_hs + lane * E);
+#pragma unroll
+            for (int x = 0; x < E / 2; ++x) raw[i][x] = src_q[x];
+        }
 
         // this warp's units: pairs warp, warp + 4, ... of [u0, u1)
         auto unit_of = [&](int k) { return u0 + 2 * (warp + kWarps * (k >> 1)) + (k & 1); };
@@ -226,18 +243,14 @@ __global__ void __launch_bounds__(kThreads, StepCfg<D, BITS, NT>::CTAS) attn_ste
 
         // Queries as f16 B fragments, a warp per row: scaled by a power of two to a maximum in [2^12, 2^13),
         // features in the order in which the key codes unpack; per group sum q and 1024 sum q (1 or 1/16).
-        for (int r = warp; r < C::ROWS; r += kWarps) {
-            constexpr int E = D / 32;
+#pragma unroll
+        for (int qi = 0; qi < QROWS; ++qi) {
+            const int r = warp + qi * kWarps;
             float q[E];
             uint32_t big = 0;
-            const int rr = min(r, nrows - 1);
-            const uint16_t* src_q = a.q + (int64_t)(s.q0 + rr / a.group) * a.q_ts + (int64_t)(h * a.group + rr % a.group) * a.q_hs + lane * E;
-            uint32_t raw[E / 2];
-#pragma unroll
-            for (int i = 0; i < E / 2; ++i) raw[i] = reinterpret_cast<const uint32_t*>(src_q)[i];
 #pragma unroll
             for (int i = 0; i < E; ++i) {
-                q[i] = r < nrows ? bf16_bits_to_f32(i & 1 ? raw[i / 2] >> 16 : raw[i / 2] & 0xffffu) : 0.f;
+                q[i] = r < nrows ? __uint_as_float(i & 1 ? raw[qi][i / 2] & 0xffff0000u : raw[qi][i / 2] << 16) : 0.f;
                 big = max(big, __float_as_uint(q[i]) & 0x7fffffffu);
             }
             big = __reduce_max_sync(0xffffffffu, big);
@@ -568,7 +581,7 @@ __global__ void __launch_bounds__(kThreads, StepCfg<D, BITS, NT>::CTAS) attn_ste
 // (M, l): 131072 positions of 8 heads of 256 features, 4 bits, 3.9 us from the last partial row to the end of
 // the call, 6.0 with these loads one after the other.
 template <int D>
-__global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ AttnArgs a, int grid, int rows) {
+__global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ AttnArgs a, int grid, int rows, int mode) {
     constexpr int F = 16, GROUPS = 256 / F, AHEAD = 8;
     __shared__ float wgt[kStepMaxCtas * 256];
     __shared__ float4 acc_s[256];
@@ -579,7 +592,7 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ 
     const int b = blockIdx.x / a.pool.kv_heads, h = blockIdx.x % a.pool.kv_heads;
     uint32_t total = 0, from = 0;
     for (int i = tid; i < a.batch; i += 256) {
-        const uint32_t v = tile_work(seq_span(a, i)) * (uint32_t)a.pool.kv_heads;
+        const uint32_t v = tile_work(seq_span(a, i), mode) * (uint32_t)a.pool.kv_heads;
         total += v;
         if (i < b) from += v;
     }
@@ -591,7 +604,7 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ 
     total = from = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) total += sums[i].x, from += sums[i].y;
-    const uint32_t share = share_of(total, grid), vl = tile_work(s);
+    const uint32_t share = mode == kAligned ? kMinShare : share_of(total, grid), vl = tile_work(s, mode);
     const uint32_t first = from + h * vl, c0 = (first + kTileCost) / share, c1 = (first + max(vl, 1u) - 1) / share;
     pdl_wait();
     pdl_launch_dependents();
@@ -678,17 +691,19 @@ cudaError_t run_step(const AttnArgs& a, cudaStream_t stream) {
     using C = StepCfg<D, BITS, NT>;
     cudaError_t e = cudaFuncSetAttribute(attn_step_kernel<D, BITS, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)C::SMEM);
     if (e != cudaSuccess) return e;
-    // no more CTAs than the longest lengths the table can hold would occupy
-    const int tiles = a.batch * a.pool.kv_heads, sms = device_num_sms();
-    const int64_t units = (int64_t)a.table_width * a.pool.page_units, most = tiles * (units + kTileCost);
+    // no more CTAs than the longest lengths that the table can hold would occupy
+    const int tiles = a.batch * a.pool.kv_heads, ctas = device_num_sms() * C::CTAS;
+    const int64_t units = (int64_t)a.table_width * a.pool.page_units;
     // Short tables: a CTA per tile, no join and no second launch.  Two rounds of a warp's pair of units take
     // less than the join would.
-    if (units <= 4 * kWarps) return launch_attn(attn_step_kernel<D, BITS, NT>, dim3(tiles), kThreads, C::SMEM, a.pdl, stream, a, 1);
-    const int grid = (int)std::min<int64_t>((int64_t)sms * C::CTAS, (most + kMinShare - 1) / kMinShare);
-    e = launch_attn(attn_step_kernel<D, BITS, NT>, dim3(grid), kThreads, C::SMEM, a.pdl, stream, a, 0);
+    if (units <= 4 * kWarps) return launch_attn(attn_step_kernel<D, BITS, NT>, dim3(tiles), kThreads, C::SMEM, a.pdl, stream, a, (int)kWholeTiles);
+    const int64_t aligned = tiles * ((units + kTileCost + kMinShare - 1) / kMinShare);
+    const int mode = aligned <= ctas ? kAligned : kEven;
+    const int grid = (int)std::min<int64_t>(aligned, ctas);
+    e = launch_attn(attn_step_kernel<D, BITS, NT>, dim3(grid), kThreads, C::SMEM, a.pdl, stream, a, mode);
     if (e != cudaSuccess || grid == 1) return e;
-    const int parts = std::max(1, std::min(4 * sms / tiles, a.max_q * a.group * (D / 64)));
-    return launch_attn(attn_join_kernel<D>, dim3(tiles, parts), 256, 0, a.pdl, stream, a, grid, (int)C::ROWS);
+    const int parts = std::max(1, std::min(4 * device_num_sms() / tiles, a.max_q * a.group * (D / 64)));
+    return launch_attn(attn_join_kernel<D>, dim3(tiles, parts), 256, 0, a.pdl, stream, a, grid, (int)C::ROWS, mode);
 }
 
 template <int D, int BITS>
