@@ -33,8 +33,9 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kStepMaxCtas = 5;  // per SM, the most of any StepCfg
 constexpr int kThreads = kWarps * 32;
-constexpr uint32_t kTileCost = 8;    // fixed cost of a tile (queries, joining the warps), in units
+constexpr uint32_t kTileCost = 16;   // fixed cost of a tile (queries, joining the warps) among equal shares, in units
 constexpr uint32_t kMinShare = kTileCost + 2 * kWarps;  // units: one pair per warp
+constexpr uint32_t kOwnShare = 16;  // units of a CTA where no CTA has two tiles
 
 template <int D, int BITS, int NT>
 struct StepCfg {
@@ -68,13 +69,14 @@ __host__ __device__ inline StepWork step_work(float* part, int grid, int rows) {
 }
 
 __device__ __forceinline__ uint32_t units_of(int len) { return (uint32_t)((len + kKvRows - 1) / kKvRows); }
-// How the work is cut: into equal shares; a CTA per tile; or into shares of kMinShare, tiles starting at one
+// How the work is cut: into equal shares; a CTA per tile; or into shares of kOwnShare, tiles starting at one
 // (where the longest lengths that the table can hold leave CTAs enough for that: no CTA works on two tiles).
 enum : int { kEven, kWholeTiles, kAligned };
 // one tile per (sequence with new tokens and positions, kv head)
+__device__ __forceinline__ uint32_t tile_cost(int mode) { return mode == kAligned ? 0u : kTileCost; }
 __device__ __forceinline__ uint32_t tile_work(const SeqSpan& s, int mode) {
-    const uint32_t v = s.n > 0 && s.len > 0 ? units_of(s.len) + kTileCost : 0u;
-    return mode == kAligned ? (v + kMinShare - 1) / kMinShare * kMinShare : v;
+    const uint32_t v = s.n > 0 && s.len > 0 ? units_of(s.len) + tile_cost(mode) : 0u;
+    return mode == kAligned ? (v + kOwnShare - 1) / kOwnShare * kOwnShare : v;
 }
 __device__ __forceinline__ uint32_t share_of(uint32_t total, uint32_t ctas) { return max(kMinShare, (total + ctas - 1) / ctas); }
 
@@ -175,7 +177,7 @@ __global__ void __launch_bounds__(kThreads, StepCfg<D, BITS, NT>::CTAS) attn_ste
     }
     __syncthreads();
     const uint32_t total = base;
-    const uint32_t share = whole_tiles ? total / a.pool.kv_heads : mode == kAligned ? kMinShare : share_of(total, gridDim.x);
+    const uint32_t share = whole_tiles ? total / a.pool.kv_heads : mode == kAligned ? kOwnShare : share_of(total, gridDim.x);
     const StepWork work = step_work(a.part, gridDim.x, C::ROWS);
     const uint64_t w_begin = (uint64_t)(whole_tiles ? (int)blockIdx.x % a.pool.kv_heads : (int)blockIdx.x) * share;
     const uint32_t w_end = (uint32_t)min((uint64_t)total, w_begin + share);
@@ -194,7 +196,8 @@ __global__ void __launch_bounds__(kThreads, StepCfg<D, BITS, NT>::CTAS) attn_ste
         const uint32_t in = w0 - pre[lo];
         const int h = (int)(in / vl);
         const uint32_t v0 = in - h * vl, v1 = min(vl, v0 + (w_end - w0));
-        const int u0 = (int)(max(v0, kTileCost) - kTileCost), u1 = (int)min(nu, max(v1, kTileCost) - kTileCost);
+        const uint32_t cost = tile_cost(mode);
+        const int u0 = (int)(max(v0, cost) - cost), u1 = (int)min(nu, max(v1, cost) - cost);
         const bool whole = u0 == 0 && u1 == (int)nu;
         const int slot = 2 * (int)blockIdx.x + (w0 == (uint32_t)w_begin ? 0 : 1);
         w0 += v1 - v0;
@@ -604,13 +607,43 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ 
     total = from = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) total += sums[i].x, from += sums[i].y;
-    const uint32_t share = mode == kAligned ? kMinShare : share_of(total, grid), vl = tile_work(s, mode);
-    const uint32_t first = from + h * vl, c0 = (first + kTileCost) / share, c1 = (first + max(vl, 1u) - 1) / share;
+    const uint32_t share = mode == kAligned ? kOwnShare : share_of(total, grid), vl = tile_work(s, mode);
+    const uint32_t first = from + h * vl, c0 = (first + tile_cost(mode)) / share, c1 = (first + max(vl, 1u) - 1) / share;
     pdl_wait();
     pdl_launch_dependents();
     if (vl == 0 || c0 == c1) return;  // nothing, or one CTA did all of it
     const uint32_t n = c1 - c0 + 1;
     auto slot_of = [&](uint32_t i) { return 2 * (c0 + i) + ((uint64_t)(c0 + i) * share >= first ? 0 : 1); };
+    auto put = [&](int row, int at, float4 x, float sum) {
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        uint16_t* y = a.out + ((int64_t)(s.q0 + row / a.group) * a.heads + h * a.group + row % a.group) * D + at * 4;
+        *reinterpret_cast<uint2*>(y) = make_uint2(bf16x2_of(x.x * inv, x.y * inv), bf16x2_of(x.z * inv, x.w * inv));
+    };
+    if (n <= AHEAD) {  // few partial rows: four features of a row per thread, all partial rows at once
+        for (int i = blockIdx.y * 256 + tid; i < s.n * a.group * (D / 4); i += gridDim.y * 256) {
+            const int row = i / (D / 4), at = i % (D / 4);
+            float2 e[AHEAD];
+            float4 v[AHEAD], acc = make_float4(0.f, 0.f, 0.f, 0.f);
+            float mx = -INFINITY, sum = 0.f;
+#pragma unroll
+            for (int k = 0; k < AHEAD; ++k) {
+                const int64_t from_row = (int64_t)slot_of(k) * rows + row;
+                e[k] = k < n ? work.ml[from_row] : make_float2(-INFINITY, 0.f);
+                v[k] = k < n ? reinterpret_cast<const float4*>(work.o)[from_row * (D / 4) + at] : acc;
+            }
+#pragma unroll
+            for (int k = 0; k < AHEAD; ++k) mx = fmaxf(mx, e[k].x);
+            if (mx == -INFINITY) mx = 0.f;
+#pragma unroll
+            for (int k = 0; k < AHEAD; ++k) {
+                const float w = ex2(e[k].x - mx);
+                sum += w * e[k].y;
+                acc.x += w * v[k].x, acc.y += w * v[k].y, acc.z += w * v[k].z, acc.w += w * v[k].w;
+            }
+            put(row, at, acc, sum);
+        }
+        return;
+    }
     const int f = tid % F, grp = tid / F;
     for (int part = blockIdx.y; part < s.n * a.group * (D / 64); part += gridDim.y) {
         const int row = part / (D / 64), fo = part % (D / 64) * 16 + f;
@@ -662,9 +695,7 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ 
                 const float4 x = acc_s[i * F + f];
                 acc.x += x.x, acc.y += x.y, acc.z += x.z, acc.w += x.w;
             }
-            const float inv = sum == 0.f ? 0.f : 1.f / sum;
-            uint16_t* y = a.out + ((int64_t)(s.q0 + row / a.group) * a.heads + h * a.group + row % a.group) * D + fo * 4;
-            *reinterpret_cast<uint2*>(y) = make_uint2(bf16x2_of(acc.x * inv, acc.y * inv), bf16x2_of(acc.z * inv, acc.w * inv));
+            put(row, fo, acc, sum);
         }
         __syncthreads();
     }
@@ -697,9 +728,9 @@ cudaError_t run_step(const AttnArgs& a, cudaStream_t stream) {
     // Short tables: a CTA per tile, no join and no second launch.  Two rounds of a warp's pair of units take
     // less than the join would.
     if (units <= 4 * kWarps) return launch_attn(attn_step_kernel<D, BITS, NT>, dim3(tiles), kThreads, C::SMEM, a.pdl, stream, a, (int)kWholeTiles);
-    const int64_t aligned = tiles * ((units + kTileCost + kMinShare - 1) / kMinShare);
-    const int mode = aligned <= ctas ? kAligned : kEven;
-    const int grid = (int)std::min<int64_t>(aligned, ctas);
+    const int64_t own = tiles * ((units + kOwnShare - 1) / kOwnShare);
+    const int mode = own <= ctas ? kAligned : kEven;
+    const int grid = (int)std::min<int64_t>(own, ctas);
     e = launch_attn(attn_step_kernel<D, BITS, NT>, dim3(grid), kThreads, C::SMEM, a.pdl, stream, a, mode);
     if (e != cudaSuccess || grid == 1) return e;
     const int parts = std::max(1, std::min(4 * device_num_sms() / tiles, a.max_q * a.group * (D / 64)));
