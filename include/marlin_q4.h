@@ -329,7 +329,9 @@ int marlin_q4_kv_read(const marlin_q4_kv_cache* cache, const int32_t* slots, int
  * q: bf16 [tokens, heads, head_dim], strides as above; out: bf16, contiguous, 16-byte aligned.
  * block_table: int32 [batch, table_width], rows table_stride elements apart; entries behind a
  * sequence's last page are not read.  heads: a multiple of kv_heads; batch at most 1024; scale > 0.
- * K and V are rounded to bf16, softmax weights too (for the tensor cores); sums are binary32.
+ * Products take f16 operands (11 bits), sums and softmax statistics are binary32.  Weights are rounded to
+ * f16.  Up to 16 rows per kv head (max_q * heads / kv_heads) keys and values enter as their codes, exact;
+ * with more rows as scale * code + bias rounded to f16, under a power of two per 16 positions.
  * A page outside the pool, a start or length outside its range sets device error 3, and the rows of that
  * sequence are void (no access leaves the buffers).
  * workspace: >= marlin_q4_paged_attention_workspace_size bytes, 256-byte aligned, any content; calls

@@ -58,7 +58,7 @@ def build_front(force: bool = False, verbose: bool = False) -> Path:
     # the shared libstdc++ by name: torch's exceptions and streams cross into this module, and some compilers
     # link theirs in statically
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", *(f"-I{i}" for i in include),
-           str(FRONT_SRC), "-o", str(FRONT), f"-L{torch / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda",
+           str(FRONT_SRC), "-o", str(FRONT), f"-L{torch / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda",
            "-l:libstdc++.so.6"]
     if verbose:
         print(" ".join(cmd), flush=True)

@@ -7,7 +7,7 @@
 #include <Python.h>
 
 #include <ATen/core/Tensor.h>
-#include <ATen/ops/empty.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -15,6 +15,7 @@
 
 #include <cmath>
 #include <initializer_list>
+#include <optional>
 
 #include "marlin_q4.h"
 
@@ -84,7 +85,7 @@ marlin_q4_kv_cache pool(const at::Tensor& data, PyObject* head_dim, PyObject* bi
     return c;
 }
 at::Tensor fresh(at::IntArrayRef shape, at::ScalarType type, const at::Tensor& like) {
-    return at::empty(shape, like.options().dtype(type));
+    return at::detail::empty_cuda(shape, type, like.device(), std::nullopt);
 }
 bool given(PyObject* o) { return o != Py_None; }
 PyObject* two(at::Tensor a, at::Tensor b) {

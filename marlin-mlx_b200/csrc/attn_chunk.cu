@@ -16,14 +16,18 @@
 // Bound: the issue slots (dequantizing about 2 instructions per cached value and tile, softmax about 3 per
 // score), then the tensor pipe (dim 256: 2048 cycles a step) and the exponentials (1024 a step).
 // Warps: 0-7 softmax and output (two threads per row, 64 columns each, who agree on M through shared
-// memory); 8 dequantize, each its own unit of a step, codes prefetched to registers straight from the pages;
-// one issues the MMAs; two go ahead, look the pages up and turn scales, biases and exponents of a step into
-// shared-memory tables.  Two tiles per CTA on the same keys (256 rows, dim 128) were measured and left out:
-// with one S buffer a tile the weights wait for both products and a step of both took 7000 cycles.  So was a
-// row per thread with two groups of softmax warps taking turns at the steps: 251 us where this takes 205.
-// Work: a planning kernel lays the tiles' steps (plus kItemCost each) of all heads end to end and cuts them
-// into equal shares, one per CTA, from the lengths on the device; a tile cut between CTAs is joined from
-// binary32 partial rows in a fixed order.
+// memory); 8 dequantize, each its own unit of a step, codes prefetched to registers straight from the pages,
+// and put the next tile's queries in while the last one's rows leave; one issues the MMAs; two go ahead, look
+// the pages up and turn scales, biases and exponents of a step into shared-memory tables.  Measured (512 rows
+// of 32 heads on 8 of 128, 4 bits, 16384 positions): 193 us, a step of a tile 3150 cycles, of which the weights
+// take 1650 and the issue slots are 61 % busy.  Left out, measured on the same: two tiles per CTA on the same
+// keys (with one S buffer a tile the weights wait for both products) 235 us where this took 198; a row per
+// thread, two groups of softmax warps taking turns at the steps, 239; weights formed before the other half's
+// maximum is known and again if it grew, 209 (its registers spill).
+// Work: a planning kernel (3.5 us) lays the tiles' steps (plus kItemCost each) of all heads end to end and cuts
+// them into equal shares, one per CTA, from the lengths on the device; a tile cut between CTAs is joined from
+// binary32 partial rows in a fixed order.  kItemCost: 2048 rows of 8 heads on 2 of 256 took 58, 52.5, 50, 52 and
+// 54 us at 1, 2, 3, 4 and 6 steps.
 #include <algorithm>
 
 #include "attn_common.cuh"
@@ -919,8 +923,8 @@ __global__ void __launch_bounds__(ChunkCfg<D, BITS>::THREADS, 1)
 template <int D>
 __global__ void __launch_bounds__(256) attn_chunk_join_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ ChunkWork work) {
     constexpr int AT = 2;  // most cut tiles have two parts
-    const bool any = blockIdx.x < work.head[0];
-    const uint32_t share = work.head[1];
+    const bool any = blockIdx.x < __ldcg(&work.head[0]);
+    const uint32_t share = __ldcg(&work.head[1]);
     const Cut c = any ? work.cuts[blockIdx.x] : Cut{};
     const SeqSpan s = seq_span(a, c.b);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n = c.c1 - c.c0 + 1;

@@ -20,8 +20,14 @@
 // ring of units fed by bulk copies (one contiguous unit per copy) and takes every fourth pair of units of
 // its CTA's range, with its own M, sums and O; the four warps are joined once at the end of a range in
 // shared memory.  The tiles' work, in units plus kTileCost for a tile's fixed cost, is laid end to end
-// and cut into equal shares, one per CTA, so that lengths of any mix load the SMs evenly; a tile that
+// and cut into equal shares, one per CTA, so that lengths of any mix load the SMs evenly; where CTAs are
+// plenty each tile starts at one of its own, since a second tile costs its CTA 4 us more.  A tile that
 // several CTAs touched is joined by a second kernel from their partial rows, in a fixed order.
+// Measured, both kernels: one row of 8 heads over 131072 positions (2 kv heads of 256, 4 bits, 75.5 MB) 29.5 us,
+// 2.6 TB/s: 3.8 to the first unit, 16 over the units (4.7 TB/s), 1.5 joining the warps, 3.9 the second kernel;
+// 32 sequences of up to 6000 positions (32 heads on 8 of 128, 8 bits, 54.7 MB) 24.9 us; 6 sequences of up to 2500,
+// four new tokens each (8 heads on 2 of 128, 4 bits) 12.6 us (17.2 in equal shares with query rows loaded one
+// after another); up to 256 positions, one kernel, 4.3 us.
 #include <algorithm>
 
 #include "attn_common.cuh"
