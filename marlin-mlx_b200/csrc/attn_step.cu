@@ -265,24 +265,45 @@ __global__ void __launch_bounds__(kThreads, StepCfg<D, BITS, NT>::CTAS) attn_ste
             big = __reduce_max_sync(0xffffffffu, big);
             const int ex = max((int)(big >> 23) - 127, -100);
             const float f = pow2i(12 - ex);
-            float sum = 0.f, off = 0.f;
-            uint16_t* qh = reinterpret_cast<uint16_t*>(qf);
+            // where a feature goes: step st of its group, lane (r & 7) * 4 + tt, register reg, half; the four
+            // numbers of a step and lane are stored at once
+            float sum = 0.f, off = 0.f, y[E];
 #pragma unroll
             for (int i = 0; i < E; ++i) {
-                const int d = lane * E + i, grp = d >> 6, tt = (d >> 4) & 3, n = d & 15;
                 const float x = q[i] * f;
-                int st, reg, half;
-                float y = x;
-                if (BITS == 4) {  // word n / 8: nibble pairs (j, j + 4), odd j left in place (16-fold)
-                    st = (n >> 3) * 2 + ((n >> 1) & 1), reg = n & 1, half = (n >> 2) & 1;
-                    if (n & 1) y = x * 0.0625f;
-                } else {
-                    st = n >> 2, reg = (n >> 1) & 1, half = n & 1;
-                }
-                const uint16_t bits = (uint16_t)f16x2_of(y, 0.f);
-                qh[((((r >> 3) * G + grp) * 4 + st) * 32 + (r & 7) * 4 + tt) * 4 + reg * 2 + half] = bits;
+                y[i] = BITS == 4 && (i & 1) ? x * 0.0625f : x;  // odd nibbles stay in place (16-fold)
                 sum += x;
-                off += y;
+                off += y[i];
+            }
+            const int d = lane * E;
+            auto at = [&](int st) { return (((r >> 3) * G + (d >> 6)) * 4 + st) * 32 + (r & 7) * 4 + ((d >> 4) & 3); };
+            if constexpr (E == 8) {
+                const int st = (lane & 1) * 2;
+                if (BITS == 4) {  // word n / 8: nibble pairs (j, j + 4)
+                    qf[at(st)] = make_uint2(f16x2_of(y[0], y[4]), f16x2_of(y[1], y[5]));
+                    qf[at(st + 1)] = make_uint2(f16x2_of(y[2], y[6]), f16x2_of(y[3], y[7]));
+                } else {
+                    qf[at(st)] = make_uint2(f16x2_of(y[0], y[1]), f16x2_of(y[2], y[3]));
+                    qf[at(st + 1)] = make_uint2(f16x2_of(y[4], y[5]), f16x2_of(y[6], y[7]));
+                }
+            } else if constexpr (E == 4 && BITS == 8) {
+                qf[at(lane & 3)] = make_uint2(f16x2_of(y[0], y[1]), f16x2_of(y[2], y[3]));
+            } else if constexpr (E == 4) {  // the other half of each pair is the neighbour's
+                const bool odd = lane & 1;
+                const uint32_t a01 = f16x2_of(y[0], y[1]), a23 = f16x2_of(y[2], y[3]);
+                const uint32_t got = __shfl_xor_sync(0xffffffffu, odd ? a01 : a23, 1);
+                const uint32_t lo = odd ? got : a01, hi = odd ? a23 : got;
+                qf[at(lane & 3)] = make_uint2(__byte_perm(lo, hi, 0x5410), __byte_perm(lo, hi, 0x7632));
+            } else {
+                const uint32_t two = f16x2_of(y[0], y[1]);
+                const int n = d & 15;
+                if (BITS == 8) {
+                    reinterpret_cast<uint32_t*>(qf + at(n >> 2))[(n >> 1) & 1] = two;
+                } else {
+                    uint16_t* qh = reinterpret_cast<uint16_t*>(qf + at((n >> 3) * 2 + ((n >> 1) & 1))) + ((n >> 2) & 1);
+                    qh[0] = (uint16_t)two;
+                    qh[2] = (uint16_t)(two >> 16);
+                }
             }
 #pragma unroll
             for (int o = 1; o < 64 / E; o <<= 1) {
