@@ -26,7 +26,7 @@
 // Measured, both kernels: one row of 8 heads over 131072 positions (2 kv heads of 256, 4 bits, 75.5 MB) 29.5 us,
 // 2.6 TB/s: 3.8 to the first unit, 16 over the units (4.7 TB/s), 1.5 joining the warps, 3.9 the second kernel;
 // 32 sequences of up to 6000 positions (32 heads on 8 of 128, 8 bits, 54.7 MB) 24.9 us; 6 sequences of up to 2500,
-// four new tokens each (8 heads on 2 of 128, 4 bits) 12.6 us (17.2 in equal shares with query rows loaded one
+// four new tokens each (8 heads on 2 of 128, 4 bits) 12.2 us (17.2 in equal shares with query rows loaded one
 // after another); up to 256 positions, one kernel, 4.3 us.
 #include <algorithm>
 
