@@ -19,11 +19,12 @@
 // memory); 8 dequantize, each its own unit of a step, codes prefetched to registers straight from the pages,
 // and put the next tile's queries in while the last one's rows leave; one issues the MMAs; two go ahead, look
 // the pages up and turn scales, biases and exponents of a step into shared-memory tables.  Measured (512 rows
-// of 32 heads on 8 of 128, 4 bits, 16384 positions): 193 us, a step of a tile 3150 cycles, of which the weights
+// of 32 heads on 8 of 128, 4 bits, 16384 positions): 190 us, a step of a tile 3100 cycles, of which the weights
 // take 1650 and the issue slots are 61 % busy.  Left out, measured on the same: two tiles per CTA on the same
 // keys (with one S buffer a tile the weights wait for both products) 235 us where this took 198; a row per
 // thread, two groups of softmax warps taking turns at the steps, 239; weights formed before the other half's
-// maximum is known and again if it grew, 209 (its registers spill).
+// maximum is known and again if it grew, 209 (its registers spill).  A barrier's wait costs some 150 cycles even
+// when its phase is over, so two are tried at once (193 us one after the other).
 // Work: a planning kernel (3.5 us) lays the tiles' steps (plus kItemCost each) of all heads end to end and cuts
 // them into equal shares, one per CTA, from the lengths on the device; a tile cut between CTAs is joined from
 // binary32 partial rows in a fixed order.  kItemCost: 2048 rows of 8 heads on 2 of 256 took 58, 52.5, 50, 52 and
@@ -263,6 +264,12 @@ __device__ __forceinline__ bool elect_one() {
     uint32_t p;
     asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
     return p;
+}
+// Both waits at once where neither has to wait
+__device__ __forceinline__ bool warp_wait_both(uint64_t* b0, uint32_t p0, uint64_t* b1, uint32_t p1, volatile int* abort) {
+    const bool r0 = mbar_try_wait(b0, p0), r1 = mbar_try_wait(b1, p1);
+    if (__all_sync(0xffffffffu, r0 && r1)) return true;
+    return warp_wait<true>(b0, p0, abort) && warp_wait<true>(b1, p1, abort);
 }
 // the two warps of a TMEM lane quarter
 __device__ __forceinline__ void pair_barrier(int quarter) { asm volatile("bar.sync %0, 64;" ::"r"(quarter + 1) : "memory"); }
@@ -519,7 +526,7 @@ __global__ void __launch_bounds__(ChunkCfg<D, BITS>::THREADS, 1)
             float m = -INFINITY, l = 0.f;
             for (int j = 0; j < n; ++j) {
                 const uint32_t gj = base + j, sl = gj % kRing;
-                ok = ok && warp_wait<true>(&efull[sl], (gj / kRing) & 1, abort) && warp_wait<true>(&sfull[gj % SB], (gj / SB) & 1, abort);
+                ok = ok && warp_wait_both(&efull[sl], (gj / kRing) & 1, &sfull[gj % SB], (gj / SB) & 1, abort);
                 if (!ok) {  // on an abort the pair still meets at its barrier, once a step
                     pair_barrier(quarter);
                     if (lane == 0) mbar_arrive(&efree[sl]);
@@ -778,9 +785,10 @@ __global__ void __launch_bounds__(ChunkCfg<D, BITS>::THREADS, 1)
                     const uint64_t qd0 = umma_desc_sw128(sq), kd0 = umma_desc_sw128(sk), vd0 = umma_desc_mn_sw128(sv, kKeys * 128);
                     auto qk = [&](int j) {
                         const uint32_t gj = base + j, st = gj % NB;
-                        if (!warp_wait<true>(&kfull[st], (gj / NB) & 1, abort)) return false;
                         // S of step j goes where P of step j - SB stands: that product has to be done
-                        if (gj >= SB && !warp_wait<true>(&pdone[gj % SB], (gj / SB - 1) & 1, abort)) return false;
+                        if (!(gj < SB ? warp_wait<true>(&kfull[st], (gj / NB) & 1, abort)
+                                      : warp_wait_both(&kfull[st], (gj / NB) & 1, &pdone[gj % SB], (gj / SB - 1) & 1, abort)))
+                            return false;
                         tc_fence_after();
                         const uint64_t kd = kd0 + (uint64_t)((st * C::KB) >> 4);
                         const uint32_t d = tmem + (gj % SB) * kKeys;
@@ -802,7 +810,7 @@ __global__ void __launch_bounds__(ChunkCfg<D, BITS>::THREADS, 1)
                     for (int j = 0; j < n && ok; ++j) {
                         if (j + 1 < n && !(ok = qk(j + 1))) break;
                         const uint32_t gj = base + j, st = gj % NB;
-                        ok = warp_wait<true>(&vfull[st], (gj / NB) & 1, abort) && warp_wait<true>(&pfull[gj % SB], (gj / SB) & 1, abort);
+                        ok = warp_wait_both(&vfull[st], (gj / NB) & 1, &pfull[gj % SB], (gj / SB) & 1, abort);
                         if (!ok) break;
                         tc_fence_after();
                         const uint64_t vd = vd0 + (uint64_t)((st * C::KB) >> 4);
