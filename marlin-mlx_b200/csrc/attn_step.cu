@@ -23,10 +23,10 @@
 // and cut into equal shares, one per CTA, so that lengths of any mix load the SMs evenly; where CTAs are
 // plenty each tile starts at one of its own, since a second tile costs its CTA 4 us more.  A tile that
 // several CTAs touched is joined by a second kernel from their partial rows, in a fixed order.
-// Measured, both kernels: one row of 8 heads over 131072 positions (2 kv heads of 256, 4 bits, 75.5 MB) 29.5 us,
-// 2.6 TB/s: 3.8 to the first unit, 16 over the units (4.7 TB/s), 1.5 joining the warps, 3.9 the second kernel;
-// 32 sequences of up to 6000 positions (32 heads on 8 of 128, 8 bits, 54.7 MB) 24.9 us; 6 sequences of up to 2500,
-// four new tokens each (8 heads on 2 of 128, 4 bits) 12.2 us (17.2 in equal shares with query rows loaded one
+// Measured, both kernels: one row of 8 heads over 131072 positions (2 kv heads of 256, 4 bits, 75.5 MB) 27.3 us,
+// 2.8 TB/s: 3.8 to the first unit, the units, 1.5 joining the warps, 3.9 the second kernel;
+// 32 sequences of up to 6000 positions (32 heads on 8 of 128, 8 bits, 54.7 MB) 20.8 us; 6 sequences of up to 2500,
+// four new tokens each (8 heads on 2 of 128, 4 bits) 12.1 us (17.2 in equal shares with query rows loaded one
 // after another); up to 256 positions, one kernel, 4.3 us.
 #include <algorithm>
 
@@ -37,7 +37,7 @@ namespace marlin {
 namespace {
 
 constexpr int kWarps = 4;
-constexpr int kStepMaxCtas = 5;  // per SM, the most of any StepCfg
+constexpr int kStepMaxCtas = 4;  // per SM, the most of any StepCfg
 constexpr int kThreads = kWarps * 32;
 constexpr uint32_t kTileCost = 16;   // fixed cost of a tile (queries, joining the warps) among equal shares, in units
 constexpr uint32_t kMinShare = kTileCost + 2 * kWarps;  // units: one pair per warp
@@ -47,8 +47,12 @@ template <int D, int BITS, int NT>
 struct StepCfg {
     static constexpr int RB = kv_row_bytes(D, BITS), G = D / 64, UB = kv_unit_bytes(D, BITS);
     static constexpr int ROWS = 8 * NT;
-    static constexpr int CTAS = NT == 2 ? (D == 256 ? 1 : D == 128 ? 3 : 4) : D == 256 ? (BITS == 4 ? 3 : 2) : D == 128 ? (BITS == 4 ? 4 : 3) : 5;
-    static constexpr int RING = D == 256 ? 3 : D == 128 ? (BITS == 4 ? 4 : 3) : (BITS == 4 ? 6 : 4);
+    // Few CTAs with many registers and deep rings: at the occupancy that 168 or 128 registers would allow, spills
+    // cost more than the warps gave (32 sequences of up to 6000 positions, 32 heads on 8, 8 bits, with two CTAs
+    // instead of three or one: dim 128 one row 20.8 us for 24.9, four rows 33 for 50; dim 256, 4 bits, four rows 52
+    // for 81; 131072 positions, dim 256, 4 bits: 27.3 for 29.5).
+    static constexpr int CTAS = D == 64 && NT == 1 ? 4 : 2;
+    static constexpr int RING = D == 256 ? (BITS == 4 ? 4 : NT == 1 ? 3 : 2) : D == 128 ? 4 : (BITS == 4 ? 6 : 4);
     static constexpr uint32_t RING_BYTES = kWarps * RING * UB;
     static constexpr uint32_t MERGE_BYTES = kWarps * ROWS * D * 4;
     static constexpr uint32_t OFF_Q = RING_BYTES > MERGE_BYTES ? RING_BYTES : MERGE_BYTES;
