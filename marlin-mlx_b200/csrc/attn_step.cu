@@ -24,7 +24,7 @@
 // plenty each tile starts at one of its own, since a second tile costs its CTA 4 us more.  A tile that
 // several CTAs touched is joined by a second kernel from their partial rows, in a fixed order.
 // Measured, both kernels: one row of 8 heads over 131072 positions (2 kv heads of 256, 4 bits, 75.5 MB) 27.3 us,
-// 2.8 TB/s: 3.8 to the first unit, the units, 1.5 joining the warps, 3.9 the second kernel;
+// 2.8 TB/s: 3.0 to the first unit, 17 over the units (4.5 TB/s), 1.2 joining the warps, 2.8 the second kernel;
 // 32 sequences of up to 6000 positions (32 heads on 8 of 128, 8 bits, 54.7 MB) 20.8 us; 6 sequences of up to 2500,
 // four new tokens each (8 heads on 2 of 128, 4 bits) 12.1 us (17.2 in equal shares with query rows loaded one
 // after another); up to 256 positions, one kernel, 4.3 us.
@@ -612,8 +612,8 @@ __global__ void __launch_bounds__(kThreads, StepCfg<D, BITS, NT>::CTAS) attn_ste
 // (row, 64 features) parts; in a block 16 lanes take 4 features each, 16 lane groups every 16th partial.
 // Bound: latency.  Where the tile was cut is worked out from the lengths while the step kernel still runs
 // (they were written before its own wait returned), and the first partial rows are loaded along with their
-// (M, l): 131072 positions of 8 heads of 256 features, 4 bits, 3.9 us from the last partial row to the end of
-// the call, 6.0 with these loads one after the other.
+// (M, l): 131072 positions of 8 heads of 256 features, 4 bits, 2.8 us from the last partial row to the end of
+// the call, 6.0 with 444 partial rows and these loads one after the other.
 template <int D>
 __global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ AttnArgs a, int grid, int rows, int mode) {
     constexpr int F = 16, GROUPS = 256 / F, AHEAD = 8;
